@@ -406,15 +406,13 @@ template <bool DYN> __global__ __launch_bounds__(512) void wgrad_phased_kernel(W
   // registers and leaves in the thief's partial slab: the combine adds the slabs in a fixed order, so only WHICH slab holds a chunk's sum
   // -- rounding -- depends on who was held.  A run of stages ("segment") is a tile's share of the token axis in the plain mode and one
   // chunk here; the staging stream runs from segment to segment, the epilogue follows a TILE.
-  // The claims are SCALAR atomics (s_atomic_add ... glc: the value before the add comes back in an SGPR and is tracked by lgkmcnt -- gfx950
-  // executes it, tools/probes/satomic_probe.hip), so they never enter the vector-memory queue whose counted waits the stream lives on.
-  // Wave 0 runs the protocol in the phases of a chunk's first two stages, one scalar memory operation per phase, issued at the phase's top and
-  // found back behind the phase's own barrier + lgkmcnt(0) (~300 ns on an idle chip, tools/probes/satomic_latency.hip: the price of a chunk): the
-  // claim on the own word; once the own share is used up, a LOOK at eight words of the tile's row (s_load_dwordx8 ... glc) for the split with the
-  // most unclaimed chunks, then the claim on that split's word.  An undisturbed launch pays one claim per chunk and, at its end, one failed
-  // claim and one look that finds nothing.  The chunk goes out through the first word of wave 0's (idle) epilogue patch (six operations at most:
-  // up to phase 1 of the second stage); all waves read it in phase 3 of the second stage -- the cursor of a four-stage chunk, the shortest
-  // the launcher allows, moves on in phase 1 of the third.
+  // The claims are vector atomics of one lane, agent scope; the compiler's wait for the returned word drains the wave's staging pieces once
+  // per claim (the price of a chunk; every other phase keeps its counted wait).  Wave 0 runs the protocol in the phases of a chunk's first two
+  // stages, one memory operation per phase, taken up behind the phase's own barrier: the claim on the own word; once the own share is used
+  // up, a LOOK at eight words of the tile's row for the split with the most unclaimed chunks, then the claim on that split's word.  An
+  // undisturbed launch pays one claim per chunk and, at its end, one failed claim and one look that finds nothing.  The chunk goes out
+  // through the first word of wave 0's (idle) epilogue patch (six operations at most: up to phase 1 of the second stage); all waves read it in
+  // phase 3 of the second stage -- the cursor of a four-stage chunk, the shortest the launcher allows, moves on in phase 1 of the third.
   constexpr bool dyn = DYN;
   const int nch = dyn ? p.chunk : 1, per_wg = dyn ? p.chunk / p.split_k : 1;
   auto chunk_begin = [&](int c) { return (int)((long)c * st_total / nch); };  // (lengths differ by at most one stage)
@@ -526,16 +524,12 @@ template <bool DYN> __global__ __launch_bounds__(512) void wgrad_phased_kernel(W
   __builtin_amdgcn_s_barrier();
 
   uint32_t r_buf = 0;
-  // ---- queue mode, wave 0: the claim protocol (see the top of the kernel).  The SGPR an atomic returns into is defined at the top of a phase and
-  // consumed behind that SAME phase's barrier + lgkmcnt(0): one variable per phase body, no join of two claims, no loop back-edge in between.
-  // The compiler believes an asm result is there at once and is free to copy the register before the value has landed (a version that let a
-  // claim fly into the next phase got exactly such copies): tools/check_satomic.py holds the listing to it -- no path from an s_atomic_add
-  // reads or writes its destination in front of an s_waitcnt lgkmcnt(0); run it after touching this kernel or the toolchain.
-  const unsigned* const q_row = dyn ? p.queue + 1 + bx * p.split_k : nullptr;  // this tile's words, one per split ([0] of the slot counts finished workgroups)
+  // ---- queue mode, wave 0: the claim protocol (see the top of the kernel)
+  unsigned* const q_row = dyn ? p.queue + 1 + bx * p.split_k : nullptr;  // this tile's words, one per split ([0] of the slot counts finished workgroups)
   bool q_need = false, own_done = false;  // this chunk's successor is still to be found; the own share is used up (persistent)
   int q_pick = -1, q_win = 0;             // the split to steal from next (-1: look first); the window of eight words the next look covers (persistent)
   auto q_publish = [&](int chunk) {
-    q_word[0] = (uint32_t)chunk;  // (every lane of wave 0 stores the same word: no per-lane branch inside the scalar protocol)
+    q_word[0] = (uint32_t)chunk;  // (every lane of wave 0 stores the same word: no per-lane branch inside the protocol)
     q_need = false;
   };
   // what this phase does for the search: 0 claim on the own word, 1 claim on q_pick's, 2 look at window q_win, -1 nothing left anywhere
@@ -553,12 +547,13 @@ template <bool DYN> __global__ __launch_bounds__(512) void wgrad_phased_kernel(W
     else if (on == sidx) own_done = true;
     else q_pick = -1;  // emptied meanwhile: look again
   };
-  auto q_land_look = [&](const u32x8& w) {  // eight words of the tile's row from split 8 * q_win: the split with the most unclaimed chunks
+  auto q_land_look = [&](uint32_t row) {  // eight words of the tile's row from split 8 * q_win: the split with the most unclaimed chunks
     int best = -1, most = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int split = 8 * q_win + j;
-      const int left = per_wg - 1 - (int)(w[j] >> 16) - (int)(w[j] & 0xffffu);
+      const uint32_t w = (uint32_t)__builtin_amdgcn_readlane((int)row, j);
+      const int left = per_wg - 1 - (int)(w >> 16) - (int)(w & 0xffffu);
       if (split < p.split_k && split != sidx && left > most) {
         most = left;
         best = split;
@@ -587,23 +582,24 @@ template <bool DYN> __global__ __launch_bounds__(512) void wgrad_phased_kernel(W
         if (draw && st == 0) q_need = true;
         static_for<NPH>([&](auto PH) {
           constexpr int P = decltype(PH)::value;
-          // queue mode, wave 0: this phase's claim, issued here and found back behind this phase's own barrier + lgkmcnt(0)
+          // queue mode, wave 0: this phase's claim, made here and taken up behind this phase's own barrier
           int q_on = -1;
           uint32_t q_ret = 0;
           int q_act = -1;
-          u32x8 q_look;
+          uint32_t q_look = 0;  // lane j: word 8 * q_win + (j & 7) of the tile's row
 #ifndef OSUD_WGQ_NOCLAIM
           if (draw && q_need) {
             q_act = q_action();
             if (q_act < 0) q_publish(0x7fffffff);
             else if (q_act == 2) {
-              const unsigned* a = q_row + 8 * q_win;
-              asm volatile("s_load_dwordx8 %0, %1, 0x0 glc" : "=s"(q_look) : "s"(a) : "memory");
+              const int split = 8 * q_win + (lane & 7);
+              q_look = __hip_atomic_load(q_row + (split < p.split_k ? split : p.split_k - 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             } else {
               q_on = q_act == 0 ? sidx : q_pick;
               q_ret = q_act == 0 ? 1u : 0x10000u;
-              const unsigned* a = q_row + q_on;
-              asm volatile("s_atomic_add %0, %1, 0x0 glc" : "+s"(q_ret) : "s"(a) : "memory");
+              uint32_t got = 0;
+              if (lane == 0) got = __hip_atomic_fetch_add(q_row + q_on, q_ret, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              q_ret = (uint32_t)__builtin_amdgcn_readfirstlane((int)got);
             }
           }
 #else  // (tuning builds: every workgroup walks its own chunks, no claims, no steals -- what the chunking alone costs)
@@ -617,14 +613,9 @@ template <bool DYN> __global__ __launch_bounds__(512) void wgrad_phased_kernel(W
           __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_barrier();
           OSUD_WG_WAIT(0);
-          if (q_act >= 0) {  // (wave 0, a claim or a look in flight: back with the wait above)
-            if (q_act == 2) {
-              asm volatile("" : "+s"(q_look));
-              q_land_look(q_look);
-            } else {
-              asm volatile("" : "+s"(q_ret));
-              q_land_claim(q_on, q_ret);
-            }
+          if (q_act >= 0) {  // (wave 0, a claim or a look was made)
+            if (q_act == 2) q_land_look(q_look);
+            else q_land_claim(q_on, q_ret);
             if (q_need && ((P >= 1 && st == 1) || q_action() < 0)) q_publish(0x7fffffff);  // out of time (six operations), or nothing left anywhere
           }
           if constexpr (P == 3) {  // (wave 0 published behind the wait of the second stage's phase 1 at the latest: two phases = four barriers ago)
