@@ -350,6 +350,67 @@ int osud_op_wgrad8(const void* P8, int ldp, const void* Q8, int ldq, int Ny, int
 int osud_op_attention_bwd(int precision, const void* qkv, const void* d_out, const void* out, const float* lse, void* dqkv,
                           int N, int T, int heads, int head_dim, float* delta_ws, osud_stream stream);
 
+/* ------------------------------------------------------------------ norms and rotary positions of queries and keys
+ * For each head x (head_dim columns) of q and of k, in one pass:
+ *   z = x * w / sqrt(mean(x^2) + eps)            (norm != 0; w: q_weight / k_weight, NULL = ones; norm == 0: z = x)
+ *   the first rot_dim columns are turned in pairs by the angle positions[row] * freqs[i], i < rot_dim / 2, and multiplied by gain:
+ *     pair i = columns (i, rot_dim / 2 + i), or (2 i, 2 i + 1) with interleaved != 0;  a' = gain (a cos - b sin), b' = gain (a sin + b cos).
+ * Rows are ld elements apart; head h starts at column h * head_dim (so a packed projection Q | K | V is read in place).  Angles
+ * are taken in 64 bits.  precision: OSUD_PREC_BF16, OSUD_PREC_F32, or OSUD_PREC_F16 (forward only).  Sums are fp32; one rounding.
+ * head_dim even, <= 128; rot_dim even, 0 .. head_dim (0: norm only; positions and freqs may be NULL); kv_heads 0: queries only.  Any row stride;
+ * 16-byte aligned rows whose rot_dim / 2 and head_dim are multiples of 8 run at memory speed, others in narrower pieces.
+ * Results may be written over the inputs (same pointers and strides). */
+typedef struct osud_rope {
+  int32_t precision, heads, kv_heads, head_dim, rot_dim, interleaved, norm;
+  int32_t float_positions;        /* 0: positions are int32, 1: float (times in ms) */
+  float eps, gain;
+  int64_t rows;
+  int64_t ld_q, ld_k;             /* elements between rows of q, k */
+  int64_t ld_q_out, ld_k_out;     /* ... of the results */
+  int64_t ld_dq, ld_dk;           /* ... of the upstream gradients (backward) */
+  const void* positions;          /* (rows) */
+  const double* freqs;            /* (rot_dim / 2), radians per position */
+  const float *q_weight, *k_weight;
+} osud_rope;
+int osud_op_qk_norm_rope(const osud_rope* r, const void* q, const void* k, void* q_out, void* k_out, osud_stream stream);
+/* d_q_out, d_k_out = gradients of the results; q, k = the forward's inputs; dq, dk (strides ld_q_out, ld_k_out) and, unless ws is NULL, the
+ * weight gradients dq_weight, dk_weight (head_dim; either may be NULL), summed in a fixed order.  ws: osud_op_qk_norm_rope_ws floats. */
+int osud_op_qk_norm_rope_bwd(const osud_rope* r, const void* d_q_out, const void* d_k_out, const void* q, const void* k, void* dq, void* dk,
+                             float* dq_weight, float* dk_weight, float* ws, size_t ws_floats, osud_stream stream);
+size_t osud_op_qk_norm_rope_ws(int head_dim);
+
+/* ------------------------------------------------------------------ attention over packed documents
+ * A batch is n_docs documents one after the other: document d has the query rows q_begin[d] .. q_begin[d + 1] - 1 and the key / value rows
+ * k_begin[d] .. k_begin[d + 1] - 1 (DEVICE arrays, int32, not decreasing; queries and keys of one document may differ in number: query i of
+ * nq stands at position nk - nq + i of its nk keys).  No pair of different documents is formed.  Query head h reads key head h / (heads / kv_heads).
+ *   s = scale * q.k;   cap > 0: s = cap * tanh(s / cap);   slopes: s -= slopes[h] * |position - key|;
+ *   key j is visible to position i if  j < prefix[d]  or  i - left <= j <= i + right   (left, right < 0: no bound; prefix NULL: 0);
+ *   out = softmax over the visible keys of s, times v;   lse = log sum exp(s).
+ * A row without a visible key: out 0, lse -inf, gradients 0.  Rows that belong to no document are neither read nor written.  Masked scores are
+ * replaced, not added to, and documents never share a tile: what lies in another document or behind the last one has no influence, NaN included;
+ * a NaN or infinity in a key or value row of the SAME document may reach every row whose 64-key block holds it.
+ * Offsets out of range or out of order are clamped: results of those documents are undefined, no access leaves the tensors.
+ * precision: OSUD_PREC_BF16, OSUD_PREC_F32, or OSUD_PREC_F16 (forward only).  head_dim: a multiple of 8, <= 128.  Pointers 16-byte aligned,
+ * row strides multiples of 16 bytes, head h at column h * head_dim. */
+typedef struct osud_doc_attention {
+  int32_t precision, heads, kv_heads, head_dim;
+  int32_t n_docs, rows_q, rows_k; /* rows of the tensors */
+  int32_t left, right;
+  int32_t max_q, max_k;           /* longest document, where known (0: not): only the split of the work depends on them, not the result's validity */
+  float scale, cap;
+  int64_t ld_q, ld_k, ld_v, ld_out, ld_d_out, ld_dq, ld_dk, ld_dv;
+  const int32_t *q_begin, *k_begin; /* (n_docs + 1) */
+  const int32_t* prefix;            /* (n_docs) or NULL */
+  const float* slopes;              /* (heads) or NULL */
+} osud_doc_attention;
+/* lse (heads, rows_q) or NULL.  ws: osud_op_doc_attention_ws(a, 0) floats; with less (or NULL) the key axis is split into fewer parts. */
+int osud_op_doc_attention(const osud_doc_attention* a, const void* q, const void* k, const void* v, void* out, float* lse, float* ws,
+                          size_t ws_floats, osud_stream stream);
+/* out, lse as the forward left them.  ws: osud_op_doc_attention_ws(a, 1) floats (at least 2 * heads * rows_q).  No atomics: the same bits every time. */
+int osud_op_doc_attention_bwd(const osud_doc_attention* a, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                              const void* d_out, void* dq, void* dk, void* dv, float* ws, size_t ws_floats, osud_stream stream);
+size_t osud_op_doc_attention_ws(const osud_doc_attention* a, int backward);
+
 #ifdef __cplusplus
 }
 #endif

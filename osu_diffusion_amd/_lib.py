@@ -38,6 +38,22 @@ class DitCfg(C.Structure):
                                           "learn_sigma", "precision")]
 
 
+class Rope(C.Structure):
+    """`osud_rope` of include/osud.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("precision", "heads", "kv_heads", "head_dim", "rot_dim", "interleaved", "norm", "float_positions")]
+                + [("eps", C.c_float), ("gain", C.c_float)]
+                + [(n, C.c_int64) for n in ("rows", "ld_q", "ld_k", "ld_q_out", "ld_k_out", "ld_dq", "ld_dk")]
+                + [(n, C.c_void_p) for n in ("positions", "freqs", "q_weight", "k_weight")])
+
+
+class DocAttention(C.Structure):
+    """`osud_doc_attention` of include/osud.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("precision", "heads", "kv_heads", "head_dim", "n_docs", "rows_q", "rows_k", "left", "right", "max_q", "max_k")]
+                + [("scale", C.c_float), ("cap", C.c_float)]
+                + [(n, C.c_int64) for n in ("ld_q", "ld_k", "ld_v", "ld_out", "ld_d_out", "ld_dq", "ld_dk", "ld_dv")]
+                + [(n, C.c_void_p) for n in ("q_begin", "k_begin", "prefix", "slopes")])
+
+
 class NativeError(RuntimeError):
     """A libosud call failed (HIP error, missing parameter, unsupported configuration)."""
 
@@ -99,6 +115,12 @@ _SIGNATURES = {
     "osud_op_attention": (_i, [_i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "osud_op_wgrad": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "osud_op_wgrad8": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp, _vp, _vp]),
+    "osud_op_qk_norm_rope": (_i, [C.POINTER(Rope), _vp, _vp, _vp, _vp, _vp]),
+    "osud_op_qk_norm_rope_bwd": (_i, [C.POINTER(Rope), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "osud_op_qk_norm_rope_ws": (_sz, [_i]),
+    "osud_op_doc_attention": (_i, [C.POINTER(DocAttention), _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "osud_op_doc_attention_bwd": (_i, [C.POINTER(DocAttention), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "osud_op_doc_attention_ws": (_sz, [C.POINTER(DocAttention), _i]),
     "osud_op_attention_bwd": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
 }
 

@@ -1,0 +1,275 @@
+// What the kernels of attention over packed documents share (doc_attn.hip, doc_attn_bwd.hip): element types, LDS tiles, the map from a
+// workgroup to its rows, the masks, and the score.
+//
+// Rows: query head h = kvh * G + g reads key head kvh.  A document's queries x the G heads of one key head are ONE axis of "shared rows",
+// row = i * G + g: a tile of shared rows reads its key blocks once for all G heads, and the tiles of a causal mask hug the diagonal.
+#pragma once
+#include "attn_frag.h"
+
+namespace osud {
+
+struct DocAttnP {
+  const void *q, *k, *v, *o, *d_o;
+  void *out, *dq, *dk, *dv;
+  float* lse;     // [heads][rows_q], natural logarithm
+  float* delta;   // [heads][rows_q]: sum_d d_out * out (backward)
+  float* ws_o;    // forward split: [split][rows_q][heads][head_dim]; backward split: see doc_attn_bwd.hip
+  float* ws_ml;   // forward split: [split][rows_q][heads][2] = maximum (log2 domain), sum
+  size_t ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv;  // elements between rows
+  const int32_t *q_begin, *k_begin, *prefix;
+  const float* slopes;
+  int rows_q, rows_k, n_docs, heads, kv_heads, G, hd, left, right, slots, split;
+  float scale, c1 /* scale * log2(e) */, cap, c2 /* 2 scale log2(e) / cap */, cap2 /* cap * log2(e) */;
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+enum { kShapeCap = 1, kShapeSlope = 2 };
+
+// ---- element types: 16-byte operand fragments (8 halves or 4 floats per lane), one fragment pair = one contraction step
+struct DocBf16 {
+  typedef bf16_t E;
+  static constexpr int ES = 2, STEP = 16 /* rows of a transposed fragment */, BK = 64 /* keys per block */;
+  static constexpr bool kExact = false;
+  static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) { return mfma_h<false>(a, b, c); }
+  static __device__ __forceinline__ u32x4 pack(const f32x16& v, int s) { return pack8_h<false>(v, 8 * s); }
+  static __device__ __forceinline__ float dot(const u32x4& a, const u32x4& b) {
+    float r = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r = fmaf(__uint_as_float(a[i] << 16), __uint_as_float(b[i] << 16), r);
+      r = fmaf(__uint_as_float(a[i] & 0xffff0000u), __uint_as_float(b[i] & 0xffff0000u), r);
+    }
+    return r;
+  }
+};
+struct DocF16 {
+  typedef f16_t E;
+  static constexpr int ES = 2, STEP = 16, BK = 64;
+  static constexpr bool kExact = false;
+  static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) { return mfma_h<true>(a, b, c); }
+  static __device__ __forceinline__ u32x4 pack(const f32x16& v, int s) { return pack8_h<true>(v, 8 * s); }
+};
+struct DocF32 {
+  typedef float E;
+  static constexpr int ES = 4, STEP = 8, BK = 32;
+  static constexpr bool kExact = true;
+  static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ u32x4 pack(const f32x16& v, int s) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[4 * s + i]);
+    return r;
+  }
+  static __device__ __forceinline__ float dot(const u32x4& a, const u32x4& b) {
+    float r = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r = fmaf(__uint_as_float(a[i]), __uint_as_float(b[i]), r);
+    return r;
+  }
+};
+
+// ---- LDS tiles: row-major rows of RB bytes, 16-byte chunks XOR-swizzled with the row so that both kinds of read spread over the 64
+// banks: 16 rows of one chunk (rowfrag: 16 different 4-bank groups) and 4 rows x 64 bytes (one transposing read: 4 different 16-bank
+// groups).  The LDS-DMA writes lanes one after the other, so the swizzle is applied to the source address.
+template <typename T, int HDP> struct DocTile {
+  static constexpr int RB = HDP * T::ES, CPR = RB / 16;
+  static_assert(RB == 128 || RB == 192 || RB == 256 || RB == 384 || RB == 512, "tile rows of 64, 96 or 128 columns");
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (RB == 128) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);  // (row & 1 is bank bit 5 already)
+    else if constexpr (RB == 192) return (row >> 2) & 3;                         // (rows 0..3 start 48 banks apart; 12 chunks: XOR inside fours)
+    else if constexpr (RB == 384) return (row >> 1) & 7;                         // (24 chunks: XOR inside eights)
+    else return ((row & 3) << 2) | ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ int off(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
+  static __device__ __forceinline__ u32x4 rowfrag(const char* tile, int row, int chunk) {
+    return *reinterpret_cast<const u32x4*>(tile + off(row, chunk));
+  }
+  // contraction over the tile's rows r0 .. r0 + STEP - 1 for column d0 + (lane & 31), in the order in which T::pack leaves the score registers
+  static __device__ __forceinline__ u32x4 trfrag(const char* tile, int r0, int d0, int lane) {
+    if constexpr (T::ES == 2) {
+      const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+      const int colb = (d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      typedef const __attribute__((address_space(3))) char lds_char;
+      lds_char* base = (lds_char*)tile;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>((const lds_s16x4*)(base + off(row, colb >> 4) + (colb & 15))));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>((const lds_s16x4*)(base + off(row + 8, colb >> 4) + (colb & 15))));
+      const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+      u32x4 v;
+      v[0] = l2[0]; v[1] = l2[1]; v[2] = h2[0]; v[3] = h2[1];
+      return v;
+    } else {
+      const int colb = (d0 + (lane & 31)) * 4, row = r0 + 4 * (lane >> 5);
+      u32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint32_t*>(tile + off(row + i, colb >> 4) + (colb & 15));
+      return v;
+    }
+  }
+};
+
+// ---- LDS-DMA of `rows` (a multiple of 4 per wave) tile rows by one workgroup of W waves: rows first + r, r >= 0, of a matrix with row stride
+// ldb bytes; source rows past `last` read row `last` again (they are masked by index; the data stays finite where the document's is).
+// Chunks behind the head's columns are not loaded: their LDS bytes were cleared once by clear_pads.
+// A wave instruction moves 64 chunks = 1024 bytes; DocTile rows are whole numbers of chunks, so lane -> (row, chunk) is fixed per piece.
+template <typename T, int HDP, int ROWS, int W> struct DocStage {
+  using TL = DocTile<T, HDP>;
+  static constexpr int BYTES = ROWS * TL::RB, PIECES = BYTES / 1024, PER = PIECES / W;
+  static_assert(BYTES % 1024 == 0 && PIECES % W == 0, "whole pieces per wave");
+  static __device__ __forceinline__ void row_chunk(int piece, int lane, int& row, int& chunk) {
+    const int c = piece * 64 + lane;
+    row = c / TL::CPR;
+    chunk = (c - row * TL::CPR) ^ TL::swz(row);
+  }
+  // per-lane byte offsets of this wave's pieces from the tile's first row (whole tiles)
+  static __device__ __forceinline__ void offsets(int wave, int lane, uint32_t ldb, uint32_t (&vo)[PER]) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row, chunk;
+      row_chunk(wave * PER + i, lane, row, chunk);
+      vo[i] = (uint32_t)row * ldb + (uint32_t)(chunk << 4);
+    }
+  }
+  static __device__ __forceinline__ void load(const char* first /* wave-uniform: the tile's first row, this head's columns */, int valid /* rows there are, >= 1 */,
+                                              uint32_t ldb, int hd, uint32_t lds /* tile */, int wave, int lane, const uint32_t (&vo)[PER]) {
+    const int cols = hd * T::ES / 16;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int piece = wave * PER + i;
+      int row, chunk;
+      row_chunk(piece, lane, row, chunk);
+      uint32_t off = vo[i];
+      if (valid < ROWS) off = (uint32_t)(row < valid ? row : valid - 1) * ldb + (uint32_t)(chunk << 4);
+      const uint32_t dst = lds + (uint32_t)piece * 1024u;
+      if (cols == TL::CPR || chunk < cols)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(first), "s"(dst) : "memory");
+    }
+  }
+  static __device__ __forceinline__ void clear_pads(char* tile, int hd, int tid, int threads) {
+    const int cols = hd * T::ES / 16;
+    if (cols == TL::CPR) return;
+    for (int c = tid; c < ROWS * TL::CPR; c += threads) {
+      const int row = c / TL::CPR, chunk = c - row * TL::CPR;
+      if (chunk >= cols) *reinterpret_cast<uint4*>(tile + TL::off(row, chunk)) = make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// ---- a workgroup's document and rows.  Tile t of document d sits in slot floor(begin[d] * m / BM) + d + t (m shared rows per query): distinct for
+// every tile without a table, at most one unused slot per document.  64 documents are looked at per step.
+struct DocRange {
+  int q0, nq, k0, nk, pre;  // first query / key row, how many, length of the prefix
+};
+__device__ __forceinline__ int doc_clamp(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
+__device__ __forceinline__ int doc_find(const int32_t* begin, int n_docs, int rows, int m, int bm, int slot, int lane, int& tile) {
+  auto start = [&](int d) { return (int)((long)doc_clamp(begin[d], 0, rows) * m / bm) + d; };
+  int lo = 0, len = n_docs;
+  while (len > 1) {
+    const int step = (len + 63) >> 6, d = lo + lane * step;
+    const bool in = lane * step < len && start(d) <= slot;
+    int n = __popcll(__ballot(in));
+    n = n < 1 ? 1 : n;
+    const int skip = (n - 1) * step;
+    lo += skip;
+    len = len - skip < step ? len - skip : step;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  tile = __builtin_amdgcn_readfirstlane(slot - start(lo));
+  return lo;
+}
+// (offsets that are not in order or out of range give wrong results for their documents and nothing else: every row stays inside the tensors)
+__device__ __forceinline__ DocRange doc_range(const DocAttnP& p, int d) {
+  DocRange r;
+  r.q0 = doc_clamp(p.q_begin[d], 0, p.rows_q);
+  r.nq = doc_clamp(p.q_begin[d + 1], r.q0, p.rows_q) - r.q0;
+  r.k0 = doc_clamp(p.k_begin[d], 0, p.rows_k);
+  r.nk = doc_clamp(p.k_begin[d + 1], r.k0, p.rows_k) - r.k0;
+  r.pre = p.prefix != nullptr ? doc_clamp(p.prefix[d], 0, r.nk) : 0;
+  return r;
+}
+// XCD-contiguous order of `n` units: workgroup b runs on XCD b % 8 and takes the units of one contiguous eighth, so that the tiles of one
+// (document, key head) read their keys through one L2
+__device__ __forceinline__ int doc_unit(int b, int n) {
+  const int q = n >> 3, r = n & 7, xcd = b & 7, idx = b >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+// ---- masks: key j is visible to position i if j < pre or i - left <= j <= i + right (a negative bound: none)
+struct DocBand {
+  int lo, hi;
+};
+__device__ __forceinline__ DocBand doc_band(const DocAttnP& p, int pos, int nk) {  // keys [lo, hi] of one position; hi < lo: none
+  DocBand b;
+  b.lo = p.left < 0 || pos - p.left < 0 ? 0 : pos - p.left;
+  b.hi = p.right < 0 || pos + p.right > nk - 1 ? nk - 1 : pos + p.right;
+  return b;
+}
+// 0: no pair of the positions [i0, i1] and the keys [j0, j1] (cut off at nk) is visible; 2: every one is, and j1 < nk; 1: some
+__device__ __forceinline__ int doc_class(const DocAttnP& p, int i0, int i1, int j0, int j1, int nk, int pre) {
+  if (j0 >= nk) return 0;
+  const bool before = p.left >= 0 && j1 < i0 - p.left, behind = p.right >= 0 && j0 > i1 + p.right;
+  if (j0 >= pre && (before || behind)) return 0;
+  const bool band = (p.left < 0 || j0 >= i1 - p.left) && (p.right < 0 || j1 <= i0 + p.right);
+  return j1 < nk && (band || j1 < pre) ? 2 : 1;
+}
+
+// ---- scores in the log2 domain.  tanh(x) = 1 - 2 / (1 + e^(2x)): `r` = 1 / (1 + e^(2x)) is kept, 1 - tanh^2 = 4 r (1 - r).  The fp32 tier takes
+// the series below |x| = 1/4, where that form loses relative accuracy (next term: 9e-3 x^11, 2e-9).
+template <typename T> __device__ __forceinline__ float doc_capped(const DocAttnP& p, float s, float& r) {
+  r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * p.c2));
+  if constexpr (T::kExact) {
+    const float x = s * p.scale / p.cap, y = x * x;
+    const float t = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const bool small = fabsf(x) < 0.25f;
+    if (small) r = 0.5f - 0.5f * t;
+    return small ? p.cap2 * t : fmaf(-2.0f * p.cap2, r, p.cap2);
+  }
+  return fmaf(-2.0f * p.cap2, r, p.cap2);
+}
+template <typename T, int SHAPE> __device__ __forceinline__ float doc_score(const DocAttnP& p, float s, float slope2, float distance, float& r) {
+  float v;
+  if constexpr ((SHAPE & kShapeCap) != 0) v = doc_capped<T>(p, s, r);
+  else v = s * p.c1;
+  if constexpr ((SHAPE & kShapeSlope) != 0) v = fmaf(-slope2, fabsf(distance), v);
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ void doc_store4(char* p, const f32x16& v, int g, float f) {  // registers 4 g .. 4 g + 3, times f
+  if constexpr (T::ES == 4) *reinterpret_cast<float4*>(p) = make_float4(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+  else store4(reinterpret_cast<typename T::E*>(p), v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+}
+// 32 accumulator columns of a wave (lane & 31 = row of the result, d = 32 dt + 8 g + 4 half + i) -> rows of the result through a patch of LDS,
+// stored as whole 16-byte chunks, neighbouring lanes on neighbouring chunks.  row(r) = address of result row r, nullptr: not stored.
+template <typename T, int HDP, typename ROW>
+__device__ __forceinline__ void doc_store_rows(char* patch, const f32x16 (&acc)[HDP / 32], float f, int hd, int lane, ROW row) {
+  using TL = DocTile<T, HDP>;
+  const int fr = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int dt = 0; dt < HDP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int b = (dt * 32 + 8 * g + 4 * half) * T::ES;
+      doc_store4<T>(patch + TL::off(fr, b >> 4) + (b & 15), acc[dt], g, f);
+    }
+  asm volatile("" ::: "memory");  // (the LDS operations of a wave execute in order)
+  const int cols = hd * T::ES / 16;
+#pragma unroll 4
+  for (int c = lane; c < 32 * TL::CPR; c += 64) {
+    const int r = c / TL::CPR, chunk = c - r * TL::CPR;
+    char* dst = row(r);
+    if (dst != nullptr && chunk < cols) *reinterpret_cast<u32x4*>(dst + chunk * 16) = *reinterpret_cast<const u32x4*>(patch + TL::off(r, chunk));
+  }
+  asm volatile("" ::: "memory");
+}
+
+size_t doc_attn_ws(const DocAttnP& p, int prec, int max_k);   // floats of the forward's workspace (0: no split)
+size_t doc_attn_bwd_ws(const DocAttnP& p, int max_q);  // floats of the backward's: delta, lse2, parts of a split
+int launch_doc_attn(int prec, DocAttnP& p, int max_k, size_t ws_floats, hipStream_t st);
+int launch_doc_attn_bwd(int prec, DocAttnP& p, int max_q, size_t ws_floats, hipStream_t st);
+
+}  // namespace osud

@@ -1,0 +1,276 @@
+// Attention over packed documents, forward:  s = scale q.k;  s = cap tanh(s / cap);  s -= slope_h |pos_q - pos_k|;  masks;  o = softmax(s) v.
+// (Reference: nn.MultiheadAttention inside DiTBlock.forward, models.py:130-135,164-170, with the (T, T) boolean mask of sample.py:81-84.)
+//
+// One workgroup = 128 shared rows (queries x the heads of one key head, see doc_attn.h) of one document, four waves of 32 rows.  S^T = K.Q^T on
+// the 32 x 32 matrix instructions, so a lane owns one row and the softmax needs one exchange with lane ^ 32; P goes back into the matrix
+// pipe as the B operand without leaving registers; the K | V rows of the next block travel by LDS-DMA into the other half of a double
+// buffer while this block is computed, one barrier per block.  Statistics, sums and accumulators are fp32; P is rounded to the
+// element type for its product (relative 2^-9 in bf16, 2^-12 in fp16: the size of the output's own rounding), its sum is taken before.
+#include "doc_attn.h"
+#include "kernels.h"
+
+namespace osud {
+namespace {
+
+template <typename T, int HDP, int SHAPE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+  using TL = DocTile<T, HDP>;
+  constexpr int BK = T::BK, KT = BK / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  using ST = DocStage<T, HDP, BK, 4>;
+  constexpr int TILE = ST::BYTES, STAGE = 2 * TILE;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const uint32_t lds0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int frow = lane & 31, half = lane >> 5;
+
+  int u = doc_unit(blockIdx.x, gridDim.x);
+  const int sp = u % p.split;
+  u /= p.split;
+  const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);  // (last tiles first: under a causal mask they are the longest)
+  int tile;
+  const DocRange d = doc_range(p, doc_find(p.q_begin, p.n_docs, p.rows_q, p.G, 128, slot, lane, tile));
+  const long vrows = (long)d.nq * p.G;
+  const long row0 = (long)tile * 128;
+  if (tile < 0 || row0 >= vrows) return;
+
+  // this lane's row
+  const long vr = row0 + wave * 32 + frow;
+  const long vrc = vr < vrows ? vr : vrows - 1;
+  const int qi = (int)(vrc / p.G), head = kvh * p.G + (int)(vrc - (long)qi * p.G);
+  const int shift = d.nk - d.nq, pos = shift + qi;
+  const size_t qrow = (size_t)d.q0 + qi;
+  // positions of the workgroup's and of this wave's rows
+  auto pos_of = [&](long r) { return shift + (int)((r < vrows ? r : vrows - 1) / p.G); };
+  const int wg0 = pos_of(row0), wg1 = pos_of(row0 + 127);
+  const int wv0 = pos_of(row0 + wave * 32), wv1 = pos_of(row0 + wave * 32 + 31);
+  const bool alive = row0 + wave * 32 < vrows;
+
+  // the blocks to visit: those of the prefix, then those of the band
+  const int npre = (d.pre + BK - 1) / BK;
+  int bl = doc_band(p, wg0, d.nk).lo / BK;
+  const int hi = doc_band(p, wg1, d.nk).hi;
+  if (bl < npre) bl = npre;
+  const int nband = hi < 0 || hi / BK < bl ? 0 : hi / BK - bl + 1;
+  const int nblk = npre + nband;
+  int it = (int)((long)sp * nblk / p.split);
+  const int it_end = (int)((long)(sp + 1) * nblk / p.split);
+
+  const uint32_t ldkb = (uint32_t)(p.ld_k * T::ES), ldvb = (uint32_t)(p.ld_v * T::ES);
+  const char* const kbase = reinterpret_cast<const char*>(p.k) + ((size_t)d.k0 * p.ld_k + (size_t)kvh * p.hd) * T::ES;
+  const char* const vbase = reinterpret_cast<const char*>(p.v) + ((size_t)d.k0 * p.ld_v + (size_t)kvh * p.hd) * T::ES;
+  uint32_t vok[ST::PER], vov[ST::PER];
+  ST::offsets(wave, lane, ldkb, vok);
+  ST::offsets(wave, lane, ldvb, vov);
+  auto block_of = [&](int i) { return i < npre ? i : i - npre + bl; };
+  auto issue = [&](int i, int stage) {
+    const int j0 = block_of(i) * BK;
+    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, p.hd, lds0 + stage * STAGE, wave, lane, vok);
+    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, p.hd, lds0 + stage * STAGE + TILE, wave, lane, vov);
+  };
+  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, p.hd, tid, 256);
+  if (it < it_end) issue(it, 0);
+
+  const int cols = p.hd * T::ES / 16;
+  u32x4 qf[KS];
+  {
+    const char* qp = reinterpret_cast<const char*>(p.q) + (qrow * p.ld_q + (size_t)head * p.hd) * T::ES;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = u32x4{0u, 0u, 0u, 0u};
+      if (2 * ks + half < cols) qf[ks] = *reinterpret_cast<const u32x4*>(qp + (2 * ks + half) * 16);
+    }
+  }
+  float slope2 = 0.f;
+  if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[head] * kLog2e;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));  // (waited for here, not inside the loop, where it would drain the DMA)
+
+  const DocBand band = doc_band(p, pos, d.nk);
+  f32x16 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  int stage = 0;
+  for (; it < it_end; ++it) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (it + 1 < it_end) issue(it + 1, stage ^ 1);
+    const int j0 = block_of(it) * BK;
+    const char* Ks = smem + stage * STAGE;
+    const char* Vs = Ks + TILE;
+    stage ^= 1;
+    const int cls = alive ? doc_class(p, wv0, wv1, j0, j0 + BK - 1, d.nk, d.pre) : 0;
+    if (cls == 0) continue;
+    f32x16 s[KT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (2 * ks < cols) s[kt] = T::mma(TL::rowfrag(Ks, kt * 32 + frow, 2 * ks + half), qf[ks], s[kt]);
+    }
+    // scores (log2 domain), masks, block maximum
+    float mx = -INFINITY;
+    const int key_lane = j0 + 4 * half;
+    const float dist0 = (float)(pos - key_lane);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int off = kt * 32 + 8 * (r >> 2) + (r & 3);
+        float rr;
+        s[kt][r] = doc_score<T, SHAPE>(p, s[kt][r], slope2, dist0 - (float)off, rr);
+      }
+    if (cls == 1) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key_lane + kt * 32 + 8 * (r >> 2) + (r & 3);
+          const bool seen = key < d.pre || (key >= band.lo && key <= band.hi);
+          s[kt][r] = seen ? s[kt][r] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // The reference point moves only when a score passes it by 8 binary orders: p <= 2^8 stays far inside every type's range, and the
+    // accumulators are rescaled a few times per row instead of once per block
+    const bool up = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
+    if (__any(up)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(s[kt][r] - m_use);
+        s[kt][r] = e;
+        l_run += e;
+      }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int ss = 0; ss < 32 / T::STEP; ++ss) {
+        const u32x4 pf = T::pack(s[kt], ss);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          if (dt * 32 < p.hd) o[dt] = T::mma(TL::trfrag(Vs, kt * 32 + T::STEP * ss, dt * 32, lane), pf, o[dt]);
+      }
+  }
+  __syncthreads();  // (the stages are idle: they become the waves' patches)
+  if (!alive) return;
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  char* const patch = smem + wave * 32 * TL::RB;
+  if (p.split == 1) {
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // (no key seen: zeros)
+    if (p.lse != nullptr && half == 0 && vr < vrows)
+      p.lse[(size_t)head * p.rows_q + qrow] = l == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(l)) * kLn2;
+    doc_store_rows<T, HDP>(patch, o, inv, p.hd, lane, [&](int r) -> char* {
+      const long v = row0 + wave * 32 + r;
+      if (v >= vrows) return nullptr;
+      const int i = (int)(v / p.G);
+      return reinterpret_cast<char*>(p.out) + (((size_t)d.q0 + i) * p.ld_o + (size_t)(kvh * p.G + (int)(v - (long)i * p.G)) * p.hd) * T::ES;
+    });
+  } else {
+    if (vr < vrows) {
+      const size_t at = ((size_t)sp * p.rows_q + qrow) * p.heads + head;
+      if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * at) = make_float2(m_run, l);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = dt * 32 + 8 * g + 4 * half;
+          if (c < p.hd) *reinterpret_cast<float4*>(p.ws_o + at * p.hd + c) = make_float4(o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
+        }
+    }
+  }
+}
+
+// joins the parts of a split: one thread per (row, head, 8 columns), parts in order
+template <typename T> __global__ __launch_bounds__(256) void doc_join_kernel(DocAttnP p) {
+  const int cpr = p.hd / 8;
+  const size_t n = (size_t)p.rows_q * p.heads;
+  const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t at = idx / cpr;
+  const int c = (int)(idx - at * cpr) * 8;
+  if (at >= n) return;
+  const size_t row = at / p.heads;
+  const int head = (int)(at - row * p.heads);
+  const int last = doc_clamp(p.q_begin[p.n_docs], 0, p.rows_q);
+  if ((long)row >= last || (long)row < doc_clamp(p.q_begin[0], 0, p.rows_q)) return;  // (rows of no document: nothing was written for them)
+  float m = -INFINITY;
+  for (int s = 0; s < p.split; ++s) m = fmaxf(m, p.ws_ml[2 * (s * n + at)]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[8] = {};
+  for (int s = 0; s < p.split; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (s * n + at));
+    const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mu);
+    l = fmaf(ml.y, w, l);
+    float v[8];
+    load8(p.ws_o + (s * n + at) * p.hd + c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+  }
+  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] *= inv;
+  store8(reinterpret_cast<typename T::E*>(p.out) + row * p.ld_o + (size_t)head * p.hd + c, acc);
+  if (c == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <typename T, int HDP, int SHAPE> int run_doc_attn(const DocAttnP& p, hipStream_t st) {
+  constexpr int lds = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * DocTile<T, HDP>::RB;
+  constexpr int bytes = lds > patch ? lds : patch;
+  const auto kernel = doc_attn_kernel<T, HDP, SHAPE>;
+  if (bytes > 64 * 1024) OSUD_BIG_LDS_ONCE(kernel);
+  kernel<<<dim3((unsigned)(p.slots * p.kv_heads * p.split)), 256, bytes, st>>>(p);
+  OSUD_HIP(hipGetLastError());
+  if (p.split > 1) {
+    const size_t items = (size_t)p.rows_q * p.heads * (p.hd / 8);
+    doc_join_kernel<T><<<dim3((unsigned)((items + 255) / 256)), 256, 0, st>>>(p);
+    OSUD_HIP(hipGetLastError());
+  }
+  return OSUD_OK;
+}
+template <typename T, int HDP> int run_doc_attn_shape(const DocAttnP& p, hipStream_t st) {
+  switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
+    case 0: return run_doc_attn<T, HDP, 0>(p, st);
+    case kShapeCap: return run_doc_attn<T, HDP, kShapeCap>(p, st);
+    case kShapeSlope: return run_doc_attn<T, HDP, kShapeSlope>(p, st);
+    default: return run_doc_attn<T, HDP, kShapeCap | kShapeSlope>(p, st);
+  }
+}
+template <typename T> int run_doc_attn_hd(const DocAttnP& p, hipStream_t st) {
+  if (p.hd <= 64) return run_doc_attn_shape<T, 64>(p, st);
+  if (p.hd <= 96) return run_doc_attn_shape<T, 96>(p, st);
+  return run_doc_attn_shape<T, 128>(p, st);
+}
+
+}  // namespace
+
+size_t doc_attn_ws(const DocAttnP&, int, int) { return 0; }
+
+int launch_doc_attn(int prec, DocAttnP& p, int max_k, size_t ws_floats, hipStream_t st) {
+  p.split = 1;
+  if (prec == OSUD_PREC_BF16) return run_doc_attn_hd<DocBf16>(p, st);
+  if (prec == OSUD_PREC_F16) return run_doc_attn_hd<DocF16>(p, st);
+  return run_doc_attn_hd<DocF32>(p, st);
+}
+
+}  // namespace osud

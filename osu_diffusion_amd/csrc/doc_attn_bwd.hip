@@ -1,0 +1,405 @@
+// Attention over packed documents, backward.  With p = exp(s - lse), dp = d_out . v, delta = sum_d d_out out (= sum_j p dp):
+//   ds = p (dp - delta) (1 - tanh^2 where capped);  dq = scale ds k;  dk = scale ds^T q;  dv = p^T d_out;  dk, dv summed over the shared heads.
+// (Reference: autograd of nn.MultiheadAttention, train.py:257.)
+//
+// Two kernels, each recomputing s and dp: the first owns query rows and walks key blocks (dq; it also writes delta and lse * log2(e) for the
+// second), the second owns keys and walks query blocks (dk, dv).  Seven products instead of the five of a single pass, but every sum
+// is taken in a fixed order: no atomics, two runs give the same bits.  p and ds are rounded to the element type for their products.
+#include "doc_attn.h"
+#include "kernels.h"
+
+namespace osud {
+namespace {
+
+// p and ds of one pair.  `v`: q.k;  lse2 = lse * log2(e)
+template <typename T, int SHAPE>
+__device__ __forceinline__ void doc_pair(const DocAttnP& p, float qk, float dp, float slope2, float distance, float lse2, float delta, bool seen, float& prob, float& ds) {
+  float r = 0.f;
+  const float v = doc_score<T, SHAPE>(p, qk, slope2, distance, r);
+  prob = seen ? __builtin_amdgcn_exp2f(v - lse2) : 0.f;
+  ds = prob * (dp - delta);
+  if constexpr ((SHAPE & kShapeCap) != 0) ds *= 4.0f * r * (1.0f - r);
+}
+
+template <typename T, int HDP, int SHAPE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 && T::ES == 4 ? 1 : 2))) void doc_attn_dq_kernel(DocAttnP p) {
+  using TL = DocTile<T, HDP>;
+  constexpr int BK = T::BK, KT = BK / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  using ST = DocStage<T, HDP, BK, 4>;
+  constexpr int TILE = ST::BYTES, STAGE = 2 * TILE;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const uint32_t lds0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int frow = lane & 31, half = lane >> 5;
+
+  const int u = doc_unit(blockIdx.x, gridDim.x);
+  const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);
+  int tile;
+  const DocRange d = doc_range(p, doc_find(p.q_begin, p.n_docs, p.rows_q, p.G, 128, slot, lane, tile));
+  const long vrows = (long)d.nq * p.G;
+  const long row0 = (long)tile * 128;
+  if (tile < 0 || row0 >= vrows) return;
+  const long vr = row0 + wave * 32 + frow;
+  const long vrc = vr < vrows ? vr : vrows - 1;
+  const int qi = (int)(vrc / p.G), head = kvh * p.G + (int)(vrc - (long)qi * p.G);
+  const int shift = d.nk - d.nq, pos = shift + qi;
+  const size_t qrow = (size_t)d.q0 + qi;
+  auto pos_of = [&](long r) { return shift + (int)((r < vrows ? r : vrows - 1) / p.G); };
+  const int wg0 = pos_of(row0), wg1 = pos_of(row0 + 127);
+  const int wv0 = pos_of(row0 + wave * 32), wv1 = pos_of(row0 + wave * 32 + 31);
+  const bool alive = row0 + wave * 32 < vrows;
+
+  const int npre = (d.pre + BK - 1) / BK;
+  int bl = doc_band(p, wg0, d.nk).lo / BK;
+  const int hi = doc_band(p, wg1, d.nk).hi;
+  if (bl < npre) bl = npre;
+  const int nblk = npre + (hi < 0 || hi / BK < bl ? 0 : hi / BK - bl + 1);
+
+  const uint32_t ldkb = (uint32_t)(p.ld_k * T::ES), ldvb = (uint32_t)(p.ld_v * T::ES);
+  const char* const kbase = reinterpret_cast<const char*>(p.k) + ((size_t)d.k0 * p.ld_k + (size_t)kvh * p.hd) * T::ES;
+  const char* const vbase = reinterpret_cast<const char*>(p.v) + ((size_t)d.k0 * p.ld_v + (size_t)kvh * p.hd) * T::ES;
+  uint32_t vok[ST::PER], vov[ST::PER];
+  ST::offsets(wave, lane, ldkb, vok);
+  ST::offsets(wave, lane, ldvb, vov);
+  auto block_of = [&](int i) { return i < npre ? i : i - npre + bl; };
+  auto issue = [&](int i, int stage) {
+    const int j0 = block_of(i) * BK;
+    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, p.hd, lds0 + stage * STAGE, wave, lane, vok);
+    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, p.hd, lds0 + stage * STAGE + TILE, wave, lane, vov);
+  };
+  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, p.hd, tid, 256);
+  if (nblk > 0) issue(0, 0);
+
+  const int cols = p.hd * T::ES / 16;
+  u32x4 qf[KS], gf[KS];
+  float delta = 0.f;
+  {
+    const size_t col = (size_t)head * p.hd;
+    const char* qp = reinterpret_cast<const char*>(p.q) + (qrow * p.ld_q + col) * T::ES;
+    const char* gp = reinterpret_cast<const char*>(p.d_o) + (qrow * p.ld_do + col) * T::ES;
+    const char* op = reinterpret_cast<const char*>(p.o) + (qrow * p.ld_o + col) * T::ES;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = gf[ks] = u32x4{0u, 0u, 0u, 0u};
+      const int c = 2 * ks + half;
+      if (c < cols) {
+        qf[ks] = *reinterpret_cast<const u32x4*>(qp + c * 16);
+        gf[ks] = *reinterpret_cast<const u32x4*>(gp + c * 16);
+        delta += T::dot(gf[ks], *reinterpret_cast<const u32x4*>(op + c * 16));
+      }
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  const size_t at = (size_t)head * p.rows_q + qrow, n_at = (size_t)p.heads * p.rows_q;
+  const float lse = p.lse[at];
+  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key seen: every p is 0)
+  if (half == 0 && vr < vrows) {
+    p.delta[at] = delta;
+    p.delta[n_at + at] = lse2;
+  }
+  float slope2 = 0.f;
+  if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[head] * kLog2e;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]), "+v"(gf[ks]));  // (waited for here, not inside the loop, where it would drain the DMA)
+
+  const DocBand band = doc_band(p, pos, d.nk);
+  f32x16 dq[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
+  for (int it = 0; it < nblk; ++it) {
+    const int stage = it & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (it + 1 < nblk) issue(it + 1, stage ^ 1);
+    const int j0 = block_of(it) * BK;
+    const char* Ks = smem + stage * STAGE;
+    const char* Vs = Ks + TILE;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int cls = alive ? doc_class(p, wv0, wv1, j0 + kt * 32, j0 + kt * 32 + 31, d.nk, d.pre) : 0;
+      if (cls == 0) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (2 * ks < cols) {
+          s = T::mma(TL::rowfrag(Ks, kt * 32 + frow, 2 * ks + half), qf[ks], s);
+          dp = T::mma(TL::rowfrag(Vs, kt * 32 + frow, 2 * ks + half), gf[ks], dp);
+        }
+      const int key_lane = j0 + kt * 32 + 4 * half;
+      const float dist0 = (float)(pos - key_lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int off = 8 * (r >> 2) + (r & 3), key = key_lane + off;
+        const bool seen = cls == 2 || key < d.pre || (key >= band.lo && key <= band.hi);
+        float prob, ds;
+        doc_pair<T, SHAPE>(p, s[r], dp[r], slope2, dist0 - (float)off, lse2, delta, seen, prob, ds);
+        s[r] = ds;
+      }
+#pragma unroll
+      for (int ss = 0; ss < 32 / T::STEP; ++ss) {
+        const u32x4 f = T::pack(s, ss);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          if (dt * 32 < p.hd) dq[dt] = T::mma(TL::trfrag(Ks, kt * 32 + T::STEP * ss, dt * 32, lane), f, dq[dt]);
+      }
+    }
+  }
+  __syncthreads();
+  if (!alive) return;
+  doc_store_rows<T, HDP>(smem + wave * 32 * TL::RB, dq, p.scale, p.hd, lane, [&](int r) -> char* {
+    const long v = row0 + wave * 32 + r;
+    if (v >= vrows) return nullptr;
+    const int i = (int)(v / p.G);
+    return reinterpret_cast<char*>(p.dq) + (((size_t)d.q0 + i) * p.ld_dq + (size_t)(kvh * p.G + (int)(v - (long)i * p.G)) * p.hd) * T::ES;
+  });
+}
+
+// One workgroup = 128 keys of one document and key head (a wave owns 32: lane = key); the shared heads one after the other, for each the
+// query blocks that see the keys.  With a split (few key tiles), part `sp` takes its share of the (head, block) list and leaves fp32 sums.
+template <typename T, int HDP, int SHAPE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 || T::ES == 4 ? 1 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
+  using TL = DocTile<T, HDP>;
+  constexpr int BQ = T::BK, QT = BQ / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  using ST = DocStage<T, HDP, BQ, 4>;
+  constexpr int TILE = ST::BYTES, STAGE = 2 * TILE + 2 * BQ * 4;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const uint32_t lds0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)smem;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int frow = lane & 31, half = lane >> 5;
+
+  int u = doc_unit(blockIdx.x, gridDim.x);
+  const int sp = u % p.split;
+  u /= p.split;
+  const int kvh = u / p.slots, slot = u - kvh * p.slots;
+  int tile;
+  const DocRange d = doc_range(p, doc_find(p.k_begin, p.n_docs, p.rows_k, 1, 128, slot, lane, tile));
+  const int j0 = tile * 128;
+  if (tile < 0 || j0 >= d.nk) return;
+  const int jw = j0 + wave * 32;  // this wave's first key
+  const bool alive = jw < d.nk;
+  const int key = jw + frow, keyc = key < d.nk ? key : d.nk - 1;
+  const int shift = d.nk - d.nq;
+
+  // queries that may see a key of the tile
+  int i_lo = 0, i_hi = d.nq - 1;
+  if (j0 >= d.pre) {
+    const int j1 = j0 + 127 < d.nk ? j0 + 127 : d.nk - 1;
+    if (p.right >= 0 && j0 - p.right - shift > i_lo) i_lo = j0 - p.right - shift;
+    if (p.left >= 0 && j1 + p.left - shift < i_hi) i_hi = j1 + p.left - shift;
+  }
+  const int b0 = i_lo / BQ, nb = i_hi < i_lo ? 0 : i_hi / BQ - b0 + 1;
+  const int total = nb * p.G;
+  int it = (int)((long)sp * total / p.split);
+  const int it_end = (int)((long)(sp + 1) * total / p.split);
+
+  const uint32_t ldqb = (uint32_t)(p.ld_q * T::ES), ldgb = (uint32_t)(p.ld_do * T::ES);
+  uint32_t voq[ST::PER], vog[ST::PER];
+  ST::offsets(wave, lane, ldqb, voq);
+  ST::offsets(wave, lane, ldgb, vog);
+  const size_t n_at = (size_t)p.heads * p.rows_q;
+  auto issue = [&](int i, int stage) {
+    const int g = i / nb, i0 = (b0 + i - g * nb) * BQ, head = kvh * p.G + g;
+    const size_t row = (size_t)d.q0 + i0;
+    const uint32_t lds = lds0 + stage * STAGE;
+    ST::load(reinterpret_cast<const char*>(p.q) + (row * p.ld_q + (size_t)head * p.hd) * T::ES, d.nq - i0, ldqb, p.hd, lds, wave, lane, voq);
+    ST::load(reinterpret_cast<const char*>(p.d_o) + (row * p.ld_do + (size_t)head * p.hd) * T::ES, d.nq - i0, ldgb, p.hd, lds + TILE, wave, lane, vog);
+    if (wave < 2 && lane < BQ) {  // wave 0: delta, wave 1: lse2 of the block's rows
+      const float* src = p.delta + (wave == 1 ? n_at : 0) + (size_t)head * p.rows_q + row;
+      const uint32_t off = (uint32_t)(i0 + lane < d.nq ? lane : d.nq - 1 - i0) * 4u;
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(src), "s"(lds + 2 * TILE + wave * BQ * 4) : "memory");
+    }
+  };
+  for (int i = 0; i < 2; ++i) {
+    ST::clear_pads(smem + i * STAGE, p.hd, tid, 256);
+    ST::clear_pads(smem + i * STAGE + TILE, p.hd, tid, 256);
+  }
+  if (it < it_end) issue(it, 0);
+
+  const int cols = p.hd * T::ES / 16;
+  u32x4 kf[KS], vf[KS];
+  {
+    const char* kp = reinterpret_cast<const char*>(p.k) + (((size_t)d.k0 + keyc) * p.ld_k + (size_t)kvh * p.hd) * T::ES;
+    const char* vp = reinterpret_cast<const char*>(p.v) + (((size_t)d.k0 + keyc) * p.ld_v + (size_t)kvh * p.hd) * T::ES;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = vf[ks] = u32x4{0u, 0u, 0u, 0u};
+      const int c = 2 * ks + half;
+      if (c < cols) {
+        kf[ks] = *reinterpret_cast<const u32x4*>(kp + c * 16);
+        vf[ks] = *reinterpret_cast<const u32x4*>(vp + c * 16);
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[ks]), "+v"(vf[ks]));
+
+  f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+  int stage = 0;
+  for (; it < it_end; ++it) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (it + 1 < it_end) issue(it + 1, stage ^ 1);
+    const int g = it / nb, i0 = (b0 + it - g * nb) * BQ;
+    float slope2 = 0.f;
+    if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[kvh * p.G + g] * kLog2e;
+    const char* Qs = smem + stage * STAGE;
+    const char* Gs = Qs + TILE;
+    const float* rows = reinterpret_cast<const float*>(Qs + 2 * TILE);  // delta [BQ], lse2 [BQ]
+    stage ^= 1;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int i = i0 + qt * 32;  // this sub-block's first query
+      if (!alive || i >= d.nq) continue;
+      int cls = doc_class(p, shift + i, shift + (i + 31 < d.nq ? i + 31 : d.nq - 1), jw, jw + 31, d.nk, d.pre);
+      if (cls == 0) continue;
+      if (i + 31 >= d.nq) cls = 1;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if (2 * ks < cols) {
+          s = T::mma(TL::rowfrag(Qs, qt * 32 + frow, 2 * ks + half), kf[ks], s);
+          dp = T::mma(TL::rowfrag(Gs, qt * 32 + frow, 2 * ks + half), vf[ks], dp);
+        }
+      const int qi0 = i + 4 * half;
+      const float dist0 = (float)(shift + qi0 - key);
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 de = *reinterpret_cast<const f32x4*>(rows + qt * 32 + 8 * q4 + 4 * half);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int off = 8 * q4 + e, pos = shift + qi0 + off;
+          bool seen = true;
+          if (cls == 1) {
+            const bool band = (p.left < 0 || key >= pos - p.left) && (p.right < 0 || key <= pos + p.right);
+            seen = qi0 + off < d.nq && key < d.nk && (band || key < d.pre);
+          }
+          float prob, ds;
+          doc_pair<T, SHAPE>(p, s[4 * q4 + e], dp[4 * q4 + e], slope2, dist0 + (float)off, ls[e], de[e], seen, prob, ds);
+          s[4 * q4 + e] = prob;
+          dp[4 * q4 + e] = ds;
+        }
+      }
+#pragma unroll
+      for (int ss = 0; ss < 32 / T::STEP; ++ss) {
+        const u32x4 pf = T::pack(s, ss), df = T::pack(dp, ss);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          if (dt * 32 < p.hd) {
+            dv[dt] = T::mma(TL::trfrag(Gs, qt * 32 + T::STEP * ss, dt * 32, lane), pf, dv[dt]);
+            dk[dt] = T::mma(TL::trfrag(Qs, qt * 32 + T::STEP * ss, dt * 32, lane), df, dk[dt]);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  if (!alive) return;
+  if (p.split == 1) {
+    char* const patch = smem + wave * 32 * TL::RB;
+    auto row = [&](void* base, size_t ld) {
+      return [=](int r) -> char* {
+        return jw + r >= d.nk ? nullptr : reinterpret_cast<char*>(base) + (((size_t)d.k0 + jw + r) * ld + (size_t)kvh * p.hd) * T::ES;
+      };
+    };
+    doc_store_rows<T, HDP>(patch, dk, p.scale, p.hd, lane, row(p.dk, p.ld_dk));
+    doc_store_rows<T, HDP>(patch, dv, 1.0f, p.hd, lane, row(p.dv, p.ld_dv));
+  } else if (key < d.nk) {
+    float* w = p.ws_o + (((size_t)sp * p.rows_k + d.k0 + key) * p.kv_heads + kvh) * 2 * p.hd;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = dt * 32 + 8 * g + 4 * half;
+        if (c < p.hd) {
+          *reinterpret_cast<float4*>(w + c) = make_float4(dk[dt][4 * g], dk[dt][4 * g + 1], dk[dt][4 * g + 2], dk[dt][4 * g + 3]);
+          *reinterpret_cast<float4*>(w + p.hd + c) = make_float4(dv[dt][4 * g], dv[dt][4 * g + 1], dv[dt][4 * g + 2], dv[dt][4 * g + 3]);
+        }
+      }
+  }
+}
+
+// sums the parts of a split, in order: one thread per 8 columns of dk | dv of one (key row, key head)
+template <typename T> __global__ __launch_bounds__(256) void doc_dkv_join_kernel(DocAttnP p) {
+  const int cpr = p.hd / 4;  // 8-column pieces of dk and dv
+  const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)p.rows_k * p.kv_heads;
+  const size_t at = idx / cpr;
+  int c = (int)(idx - at * cpr) * 8;
+  if (at >= n) return;
+  const size_t row = at / p.kv_heads;
+  const int kvh = (int)(at - row * p.kv_heads);
+  if ((long)row >= doc_clamp(p.k_begin[p.n_docs], 0, p.rows_k) || (long)row < doc_clamp(p.k_begin[0], 0, p.rows_k)) return;
+  float acc[8] = {};
+  for (int s = 0; s < p.split; ++s) {
+    float v[8];
+    load8(p.ws_o + (s * n + at) * 2 * p.hd + c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += v[e];
+  }
+  const bool is_k = c < p.hd;
+  if (is_k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= p.scale;
+  } else {
+    c -= p.hd;
+  }
+  store8(reinterpret_cast<typename T::E*>(is_k ? p.dk : p.dv) + row * (is_k ? p.ld_dk : p.ld_dv) + (size_t)kvh * p.hd + c, acc);
+}
+
+template <typename T, int HDP, int SHAPE> int run_doc_bwd(const DocAttnP& p0, hipStream_t st) {
+  using TL = DocTile<T, HDP>;
+  DocAttnP p = p0;
+  constexpr int tiles = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * TL::RB;
+  constexpr int bytes_q = tiles > patch ? tiles : patch, bytes_k = (tiles > patch ? tiles : patch) + 4 * T::BK * 4;
+  const auto kq = doc_attn_dq_kernel<T, HDP, SHAPE>;
+  const auto kk = doc_attn_dkv_kernel<T, HDP, SHAPE>;
+  if (bytes_q > 64 * 1024) OSUD_BIG_LDS_ONCE(kq);
+  if (bytes_k > 64 * 1024) OSUD_BIG_LDS_ONCE(kk);
+  p.slots = (int)((long)p.rows_q * p.G / 128) + p.n_docs;
+  kq<<<dim3((unsigned)(p.slots * p.kv_heads)), 256, bytes_q, st>>>(p);
+  OSUD_HIP(hipGetLastError());
+  p.slots = p.rows_k / 128 + p.n_docs;
+  kk<<<dim3((unsigned)(p.slots * p.kv_heads * p.split)), 256, bytes_k, st>>>(p);
+  OSUD_HIP(hipGetLastError());
+  if (p.split > 1) {
+    const size_t items = (size_t)p.rows_k * p.kv_heads * (p.hd / 4);
+    doc_dkv_join_kernel<T><<<dim3((unsigned)((items + 255) / 256)), 256, 0, st>>>(p);
+    OSUD_HIP(hipGetLastError());
+  }
+  return OSUD_OK;
+}
+template <typename T, int HDP> int run_doc_bwd_shape(const DocAttnP& p, hipStream_t st) {
+  switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
+    case 0: return run_doc_bwd<T, HDP, 0>(p, st);
+    case kShapeCap: return run_doc_bwd<T, HDP, kShapeCap>(p, st);
+    case kShapeSlope: return run_doc_bwd<T, HDP, kShapeSlope>(p, st);
+    default: return run_doc_bwd<T, HDP, kShapeCap | kShapeSlope>(p, st);
+  }
+}
+template <typename T> int run_doc_bwd_hd(const DocAttnP& p, hipStream_t st) {
+  if (p.hd <= 64) return run_doc_bwd_shape<T, 64>(p, st);
+  if (p.hd <= 96) return run_doc_bwd_shape<T, 96>(p, st);
+  return run_doc_bwd_shape<T, 128>(p, st);
+}
+
+}  // namespace
+
+size_t doc_attn_bwd_ws(const DocAttnP& p, int) { return 2 * (size_t)p.heads * p.rows_q; }
+
+int launch_doc_attn_bwd(int prec, DocAttnP& p, int max_q, size_t ws_floats, hipStream_t st) {
+  p.split = 1;
+  return prec == OSUD_PREC_BF16 ? run_doc_bwd_hd<DocBf16>(p, st) : run_doc_bwd_hd<DocF32>(p, st);
+}
+
+}  // namespace osud

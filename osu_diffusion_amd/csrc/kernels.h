@@ -207,4 +207,22 @@ int launch_step_init(int* step_state, int first, uint64_t seed, hipStream_t st, 
 int launch_step_begin(int* step_state, const int64_t* tmap_dev, int64_t* t_model, int64_t* t_index, int N,
                       hipStream_t st);
 
+// norms of queries and keys per head + rotary positions (qk_norm_rope.hip); backward: q, k = the forward's inputs, gq, gk = the gradients of its
+// outputs, qo, ko = the gradients of q, k; ws = rope_ws_floats(hd) floats (nullptr: no weight gradients)
+struct RopeP {
+  const void *q, *k, *gq, *gk;
+  void *qo, *ko;
+  size_t ld_q, ld_k, ld_gq, ld_gk, ld_qo, ld_ko;
+  const void* positions;
+  const double* freqs;
+  const float *qw, *kw;
+  float *dqw, *dkw, *ws;
+  long rows;
+  int heads, kv_heads, hd, rot;
+  bool interleaved, norm, float_positions;
+  float eps, gain;
+};
+size_t rope_ws_floats(int hd);
+int launch_qk_norm_rope(int prec, const RopeP& p, bool back, hipStream_t st);
+
 }  // namespace osud

@@ -1,0 +1,268 @@
+// Norms of queries and keys for each head and the rotation by position, in one pass over the rows, forward and backward.
+// (No counterpart in the reference: its positions enter through the sinusoidal features of models.py:199-225.)
+//   r = 1 / sqrt(mean x^2 + eps),  z = x r w;   pair (a, b) of z, angle th = position * f:  a' = gain (a cos th - b sin th),  b' = gain (a sin th + b cos th)
+//   backward: dz = the transposed rotation of the gradient;  dw = sum dz x r;  u = dz w;  dx = r (u - x r mean(u x r))
+// Memory bound: forward reads and writes every head once, backward reads x and the gradient and writes dx (r is computed again).
+//
+// A group of lanes owns one head of one row; a lane holds two chunks of W columns that form W whole pairs (half layout: columns i and
+// R + i; interleaved: 2 W neighbouring columns), so the rotation needs no exchange and the norm a few lane shuffles.  A workgroup takes
+// TPB rows: their angles first, one per lane, into LDS -- each serves all heads of its row.  position * f / 2 pi is taken in 64 bits and
+// reduced to a fraction of a turn there: at 10^6 positions a product in 32 bits is off by 0.06 radians.
+#include "common.h"
+#include "kernels.h"
+
+namespace osud {
+namespace {
+
+constexpr int kTpb = 8, kMaxHd = 128;
+
+template <int W, typename E> __device__ __forceinline__ void load_chunk(const E* p, float (&v)[W]) {
+  if constexpr (W == 8) load8(p, v);
+  else if constexpr (W == 1) v[0] = load_elem(p);
+  else loadw<W>(p, v);
+}
+template <int W, typename E> __device__ __forceinline__ void store_chunk(E* p, const float (&v)[W]) {
+  if constexpr (W == 8) store8(p, v);
+  else if constexpr (W == 1) store_elem(p, v[0]);
+  else storew<W>(p, v);
+}
+
+// cos and sin (times gain) of the rows t0 .. t0 + n - 1 into LDS, [row][R]
+__device__ __forceinline__ void rope_angles(const RopeP& p, long t0, int n, float2* table) {
+  const int R = p.rot / 2;
+  for (int i = threadIdx.x; i < n * R; i += 256) {
+    const int t = i / R, f = i - t * R;
+    const double pos = p.float_positions ? (double)reinterpret_cast<const float*>(p.positions)[t0 + t] : (double)reinterpret_cast<const int32_t*>(p.positions)[t0 + t];
+    double turn = pos * p.freqs[f] * 0.15915494309189533577;
+    turn -= rint(turn);
+    float s, c;
+    sincospif(2.0f * (float)turn, &s, &c);
+    table[i] = make_float2(c * p.gain, s * p.gain);
+  }
+}
+
+// one lane's two chunks of a head: columns ca .. ca + W - 1 and cb .. cb + W - 1
+template <int W> struct RopeLane {
+  int ca, cb, pair;
+  bool a, b, turn;
+  __device__ __forceinline__ RopeLane(const RopeP& p, int l) {
+    const int R = p.rot / 2, np = R / W;
+    turn = l < np;
+    pair = l * W;
+    if (turn) {
+      ca = p.interleaved ? 2 * pair : pair;
+      cb = p.interleaved ? 2 * pair + W : R + pair;
+      a = b = true;
+    } else {
+      ca = p.rot + 2 * W * (l - np);
+      cb = ca + W;
+      a = ca < p.hd;
+      b = cb < p.hd;
+    }
+  }
+};
+// (x[0 .. 2 W - 1] = chunk a, chunk b)  the rotation, or its transpose
+template <int W, bool BACK> __device__ __forceinline__ void rope_turn(const float2* cs, bool interleaved, float (&x)[2 * W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    float2 t = cs[i];
+    if (BACK) t.y = -t.y;
+    const float a0 = x[2 * i], b0 = x[2 * i + 1], a1 = x[i], b1 = x[W + i];
+    // (both layouts, selected by a uniform value; the half layout writes below)
+    if (interleaved) {
+      x[2 * i] = a0 * t.x - b0 * t.y;
+      x[2 * i + 1] = a0 * t.y + b0 * t.x;
+    } else {
+      x[i] = a1 * t.x - b1 * t.y;
+      x[W + i] = a1 * t.y + b1 * t.x;
+    }
+  }
+}
+
+template <typename E, int W, int GL /* lanes per head */, bool BACK>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
+  __shared__ float2 table[kTpb * (kMaxHd / 2)];
+  __shared__ float red[BACK ? 256 : 1];
+  const int l = threadIdx.x % GL, grp = threadIdx.x / GL;
+  constexpr int NG = 256 / GL;
+  const RopeLane<W> ln(p, l);
+  float dw[2][2 * W] = {};
+  const float inv_hd = 1.0f / (float)p.hd;
+  for (long c = blockIdx.x; c * kTpb < p.rows; c += gridDim.x) {
+    const long t0 = c * kTpb;
+    const int n = p.rows - t0 < kTpb ? (int)(p.rows - t0) : kTpb;
+    __syncthreads();
+    rope_angles(p, t0, n, table);
+    __syncthreads();
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int heads = part ? p.kv_heads : p.heads;
+      if (heads == 0) continue;
+      const E* const src = reinterpret_cast<const E*>(part ? p.k : p.q);
+      const E* const up = reinterpret_cast<const E*>(part ? p.gk : p.gq);
+      E* const dst = reinterpret_cast<E*>(part ? p.ko : p.qo);
+      const size_t ld = part ? p.ld_k : p.ld_q, ldg = part ? p.ld_gk : p.ld_gq, ldo = part ? p.ld_ko : p.ld_qo;
+      const float* const w = part ? p.kw : p.qw;
+      float wt[2 * W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        wt[i] = w != nullptr && ln.a ? w[ln.ca + i] : 1.f;
+        wt[W + i] = w != nullptr && ln.b ? w[ln.cb + i] : 1.f;
+      }
+      const int st = NG / heads, sh = NG - st * heads;
+      int t = grp / heads, h = grp - t * heads;
+      for (; t < n; t += st, h += sh) {
+        if (h >= heads) {
+          h -= heads;
+          if (++t >= n) break;
+        }
+        const size_t col = (size_t)h * p.hd;
+        const E* xp = src + (size_t)(t0 + t) * ld + col;
+        E* yp = dst + (size_t)(t0 + t) * ldo + col;
+        float xa[W] = {}, xb[W] = {}, x[2 * W];
+        if (ln.a) load_chunk<W>(xp + ln.ca, xa);
+        if (ln.b) load_chunk<W>(xp + ln.cb, xb);
+        float ga[W] = {}, gb[W] = {};
+        if constexpr (BACK) {
+          const E* gp = up + (size_t)(t0 + t) * ldg + col;
+          if (ln.a) load_chunk<W>(gp + ln.ca, ga);
+          if (ln.b) load_chunk<W>(gp + ln.cb, gb);
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          x[i] = xa[i];
+          x[W + i] = xb[i];
+        }
+        float r = 1.f;
+        if (p.norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+          for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+          const float v = fmaf(ss, inv_hd, p.eps);
+          r = 1.0f / sqrtf(v);
+        }
+        const float2* cs = table + t * (p.rot / 2) + ln.pair;
+        if constexpr (!BACK) {
+#pragma unroll
+          for (int i = 0; i < 2 * W; ++i) x[i] = x[i] * r * wt[i];
+          if (ln.turn) rope_turn<W, false>(cs, p.interleaved, x);
+        } else {
+          float g[2 * W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            g[i] = ga[i];
+            g[W + i] = gb[i];
+          }
+          if (ln.turn) rope_turn<W, true>(cs, p.interleaved, g);
+          if (p.norm) {
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) {
+              x[i] *= r;
+              dw[part][i] = fmaf(g[i], x[i], dw[part][i]);
+              g[i] *= wt[i];
+              dot = fmaf(g[i], x[i], dot);
+            }
+#pragma unroll
+            for (int o = GL / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+            dot *= inv_hd;
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) x[i] = r * fmaf(-x[i], dot, g[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) x[i] = g[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          xa[i] = x[i];
+          xb[i] = x[W + i];
+        }
+        if (ln.a) store_chunk<W>(yp + ln.ca, xa);
+        if (ln.b) store_chunk<W>(yp + ln.cb, xb);
+      }
+    }
+  }
+  if constexpr (BACK) {  // this workgroup's sums of the weight gradients, groups added in order: one row of ws
+    if (p.ws == nullptr) return;
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
+        __syncthreads();
+        red[threadIdx.x] = dw[part][i];
+        __syncthreads();
+        if (grp == 0 && (i < W ? ln.a : ln.b)) {
+          float s = 0.f;
+          for (int g = 0; g < NG; ++g) s += red[g * GL + l];
+          p.ws[((size_t)blockIdx.x * 2 + part) * p.hd + (i < W ? ln.ca + i : ln.cb + i - W)] = s;
+        }
+      }
+  }
+}
+
+// dw[c] = sum over the workgroups' rows, in a fixed order: 16 columns x 16 row lanes per workgroup
+__global__ __launch_bounds__(256) void rope_dw_kernel(const float* ws, int parts, int hd, float* dqw, float* dkw) {
+  __shared__ float red[16][17];
+  const int c = blockIdx.x * 16 + threadIdx.x % 16, rl = threadIdx.x / 16;
+  float s = 0.f;
+  if (c < 2 * hd)
+    for (int r = rl; r < parts; r += 16) s += ws[(size_t)r * 2 * hd + c];
+  red[rl][threadIdx.x % 16] = s;
+  __syncthreads();
+  if (rl != 0 || c >= 2 * hd) return;
+  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+  float* out = c < hd ? dqw : dkw;
+  if (out != nullptr) out[c < hd ? c : c - hd] = s;
+}
+
+constexpr int kBackGroups = 512;  // workgroups of the backward pass (two per CU): rows of ws
+
+template <typename E, int W, int GL, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
+  const long chunks = p.rows > kTpb ? (p.rows + kTpb - 1) / kTpb : 1;  // (no rows: one workgroup that leaves zeros for the weights)
+  const long grid = BACK && p.ws != nullptr ? (chunks < kBackGroups ? chunks : kBackGroups) : (chunks < (1L << 30) ? chunks : (1L << 30));
+  qk_norm_rope_kernel<E, W, GL, BACK><<<dim3((unsigned)grid), 256, 0, st>>>(p);
+  OSUD_HIP(hipGetLastError());
+  if (BACK && p.ws != nullptr) {
+    rope_dw_kernel<<<dim3((2 * p.hd + 15) / 16), 256, 0, st>>>(p.ws, (int)grid, p.hd, p.dqw, p.dkw);
+    OSUD_HIP(hipGetLastError());
+  }
+  return OSUD_OK;
+}
+template <typename E, int W, bool BACK> int run_rope_lanes(const RopeP& p, hipStream_t st) {
+  const int lanes = p.rot / 2 / W + ((p.hd - p.rot) / W + 1) / 2;
+  if (lanes <= 4) return run_rope<E, W, 4, BACK>(p, st);
+  if (lanes <= 8) return run_rope<E, W, 8, BACK>(p, st);
+  if (lanes <= 16) return run_rope<E, W, 16, BACK>(p, st);
+  if constexpr (W <= 4) {
+    if (lanes <= 32) return run_rope<E, W, 32, BACK>(p, st);
+    return run_rope<E, W, 64, BACK>(p, st);
+  }
+  return OSUD_ERR_ARG;
+}
+template <typename E, bool BACK> int run_rope_width(const RopeP& p, hipStream_t st) {
+  // the widest chunk that divides the pairs, the head, the rows' strides and the pointers
+  size_t all = (size_t)(p.rot / 2) | (size_t)p.hd | p.ld_q | p.ld_qo | reinterpret_cast<size_t>(p.q) / sizeof(E) | reinterpret_cast<size_t>(p.qo) / sizeof(E);
+  if (p.kv_heads) all |= p.ld_k | p.ld_ko | reinterpret_cast<size_t>(p.k) / sizeof(E) | reinterpret_cast<size_t>(p.ko) / sizeof(E);
+  if (BACK) all |= p.ld_gq | reinterpret_cast<size_t>(p.gq) / sizeof(E);
+  if (BACK && p.kv_heads) all |= p.ld_gk | reinterpret_cast<size_t>(p.gk) / sizeof(E);
+  if (all % 8 == 0) return run_rope_lanes<E, 8, BACK>(p, st);
+  if (all % 4 == 0) return run_rope_lanes<E, 4, BACK>(p, st);
+  if (all % 2 == 0) return run_rope_lanes<E, 2, BACK>(p, st);
+  return run_rope_lanes<E, 1, BACK>(p, st);
+}
+
+}  // namespace
+
+size_t rope_ws_floats(int hd) { return (size_t)kBackGroups * 2 * hd; }
+
+int launch_qk_norm_rope(int prec, const RopeP& p, bool back, hipStream_t st) {
+  if (back) return prec == OSUD_PREC_BF16 ? run_rope_width<bf16_t, true>(p, st) : run_rope_width<float, true>(p, st);
+  if (prec == OSUD_PREC_BF16) return run_rope_width<bf16_t, false>(p, st);
+  if (prec == OSUD_PREC_F16) return run_rope_width<f16_t, false>(p, st);
+  return run_rope_width<float, false>(p, st);
+}
+
+}  // namespace osud
