@@ -85,31 +85,43 @@ template <typename T, int HDP> struct DocTile {
     else return ((row & 3) << 2) | ((row >> 2) & 3);
   }
   static __device__ __forceinline__ int off(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
-  static __device__ __forceinline__ u32x4 rowfrag(const char* tile, int row, int chunk) {
-    return *reinterpret_cast<const u32x4*>(tile + off(row, chunk));
+  // The swizzle touches XB bits of the chunk, and row * RB has zeros there: the address of another chunk of the same row is an exclusive or of a
+  // constant and an addition that goes into the instruction's offset.  LDS addresses, per lane; a tile starts at a multiple of 256 bytes.
+  static constexpr int XB = RB == 192 ? 2 : (RB == 128 || RB == 384 ? 3 : 4), XM = (1 << XB) - 1;
+  static __device__ __forceinline__ uint32_t at_chunk(uint32_t base, int c) { return (base ^ (uint32_t)((c & XM) << 4)) + (uint32_t)((c >> XB) << (4 + XB)); }
+  // a row fragment = 16 bytes of row r0 + (lane & 31): contraction step ks, this lane's half of it
+  static __device__ __forceinline__ uint32_t row_base(int lane) { return (uint32_t)off(lane & 31, lane >> 5); }
+  static __device__ __forceinline__ u32x4 row_read(uint32_t base, int r0, int ks) {
+    typedef const __attribute__((address_space(3))) u32x4 lds_v;
+    return *(lds_v*)(size_t)(at_chunk(base, 2 * ks) + (uint32_t)(r0 * RB));
   }
-  // contraction over the tile's rows r0 .. r0 + STEP - 1 for column d0 + (lane & 31), in the order in which T::pack leaves the score registers
-  static __device__ __forceinline__ u32x4 trfrag(const char* tile, int r0, int d0, int lane) {
+  // a transposed fragment = contraction over the rows r0 .. r0 + STEP - 1 for column 32 dt + (lane & 31), in the order in which T::pack leaves
+  // the score registers (16-bit types: two transposing reads of 4 rows x 16 columns per 16 lanes; fp32: four words)
+  static __device__ __forceinline__ uint32_t tr_base(int lane) {
     if constexpr (T::ES == 2) {
-      const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-      const int colb = (d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), colb = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+      return (uint32_t)(off(row, colb >> 4) + (colb & 15));
+    } else {
+      return (uint32_t)(4 * (lane >> 5) * RB);
+    }
+  }
+  static __device__ __forceinline__ u32x4 tr_read(uint32_t base, int r0, int dt, int lane) {
+    u32x4 v;
+    if constexpr (T::ES == 2) {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      typedef const __attribute__((address_space(3))) char lds_char;
-      lds_char* base = (lds_char*)tile;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>((const lds_s16x4*)(base + off(row, colb >> 4) + (colb & 15))));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>((const lds_s16x4*)(base + off(row + 8, colb >> 4) + (colb & 15))));
+      const uint32_t lo_at = at_chunk(base, 4 * dt), hi_at = at_chunk(base ^ 32u, 4 * dt);  // (rows + 8: bit 1 of the swizzled chunk)
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)(lo_at + (uint32_t)(r0 * RB)));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)(hi_at + (uint32_t)((r0 + 8) * RB)));
       const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
-      u32x4 v;
       v[0] = l2[0]; v[1] = l2[1]; v[2] = h2[0]; v[3] = h2[1];
-      return v;
     } else {
-      const int colb = (d0 + (lane & 31)) * 4, row = r0 + 4 * (lane >> 5);
-      u32x4 v;
+      typedef const __attribute__((address_space(3))) uint32_t lds_w;
+      const int colb = (dt * 32 + (lane & 31)) * 4, row = 4 * (lane >> 5);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint32_t*>(tile + off(row + i, colb >> 4) + (colb & 15));
-      return v;
+      for (int i = 0; i < 4; ++i) v[i] = *(lds_w*)(size_t)(base + (uint32_t)((r0 + i) * RB + (((colb >> 4) ^ swz(r0 + row + i)) << 4) + (colb & 15)));
     }
+    return v;
   }
 };
 
@@ -135,9 +147,9 @@ template <typename T, int HDP, int ROWS, int W> struct DocStage {
       vo[i] = (uint32_t)row * ldb + (uint32_t)(chunk << 4);
     }
   }
+  // (cols: chunks of a head's row that are data)
   static __device__ __forceinline__ void load(const char* first /* wave-uniform: the tile's first row, this head's columns */, int valid /* rows there are, >= 1 */,
-                                              uint32_t ldb, int hd, uint32_t lds /* tile */, int wave, int lane, const uint32_t (&vo)[PER]) {
-    const int cols = hd * T::ES / 16;
+                                              uint32_t ldb, int cols, uint32_t lds /* tile */, int wave, int lane, const uint32_t (&vo)[PER]) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int piece = wave * PER + i;
@@ -150,8 +162,7 @@ template <typename T, int HDP, int ROWS, int W> struct DocStage {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(first), "s"(dst) : "memory");
     }
   }
-  static __device__ __forceinline__ void clear_pads(char* tile, int hd, int tid, int threads) {
-    const int cols = hd * T::ES / 16;
+  static __device__ __forceinline__ void clear_pads(char* tile, int cols, int tid, int threads) {
     if (cols == TL::CPR) return;
     for (int c = tid; c < ROWS * TL::CPR; c += threads) {
       const int row = c / TL::CPR, chunk = c - row * TL::CPR;
@@ -166,8 +177,8 @@ struct DocRange {
   int q0, nq, k0, nk, pre;  // first query / key row, how many, length of the prefix
 };
 __device__ __forceinline__ int doc_clamp(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
-__device__ __forceinline__ int doc_find(const int32_t* begin, int n_docs, int rows, int m, int bm, int slot, int lane, int& tile) {
-  auto start = [&](int d) { return (int)((long)doc_clamp(begin[d], 0, rows) * m / bm) + d; };
+template <int bm> __device__ __forceinline__ int doc_find(const int32_t* begin, int n_docs, int rows, int m, int slot, int lane, int& tile) {
+  auto start = [&](int d) { return (int)((unsigned)(doc_clamp(begin[d], 0, rows) * m) / (unsigned)bm) + d; };  // (rows * m < 2^31)
   int lo = 0, len = n_docs;
   while (len > 1) {
     const int step = (len + 63) >> 6, d = lo + lane * step;
@@ -191,6 +202,15 @@ __device__ __forceinline__ DocRange doc_range(const DocAttnP& p, int d) {
   r.nk = doc_clamp(p.k_begin[d + 1], r.k0, p.rows_k) - r.k0;
   r.pre = p.prefix != nullptr ? doc_clamp(p.prefix[d], 0, r.nk) : 0;
   return r;
+}
+// max / sum over lane and lane ^ 32 (v_permlane32_swap: the halves of two registers change places)
+__device__ __forceinline__ float doc_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float doc_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 // XCD-contiguous order of `n` units: workgroup b runs on XCD b % 8 and takes the units of one contiguous eighth, so that the tiles of one
 // (document, key head) read their keys through one L2
@@ -258,9 +278,9 @@ __device__ __forceinline__ void doc_store_rows(char* patch, const f32x16 (&acc)[
     }
   asm volatile("" ::: "memory");  // (the LDS operations of a wave execute in order)
   const int cols = hd * T::ES / 16;
-#pragma unroll 4
-  for (int c = lane; c < 32 * TL::CPR; c += 64) {
-    const int r = c / TL::CPR, chunk = c - r * TL::CPR;
+#pragma unroll
+  for (int it = 0; it < TL::CPR / 2; ++it) {
+    const int c = it * 64 + lane, r = c / TL::CPR, chunk = c - r * TL::CPR;
     char* dst = row(r);
     if (dst != nullptr && chunk < cols) *reinterpret_cast<u32x4*>(dst + chunk * 16) = *reinterpret_cast<const u32x4*>(patch + TL::off(r, chunk));
   }

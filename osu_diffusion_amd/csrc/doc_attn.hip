@@ -6,16 +6,18 @@
 // pipe as the B operand without leaving registers; the K | V rows of the next block travel by LDS-DMA into the other half of a double
 // buffer while this block is computed, one barrier per block.  Statistics, sums and accumulators are fp32; P is rounded to the
 // element type for its product (relative 2^-9 in bf16, 2^-12 in fp16: the size of the output's own rounding), its sum is taken before.
+#include <type_traits>
+
 #include "doc_attn.h"
 #include "kernels.h"
 
 namespace osud {
 namespace {
 
-template <typename T, int HDP, int SHAPE>
+template <typename T, int HDP, int KS, int SHAPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
-  constexpr int BK = T::BK, KT = BK / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
   constexpr int TILE = ST::BYTES, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -24,25 +26,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   const int frow = lane & 31, half = lane >> 5;
 
   int u = doc_unit(blockIdx.x, gridDim.x);
-  const int sp = u % p.split;
-  u /= p.split;
+  const int sp = p.split > 1 ? u % p.split : 0;
+  if (p.split > 1) u /= p.split;
   const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);  // (last tiles first: under a causal mask they are the longest)
   int tile;
-  const DocRange d = doc_range(p, doc_find(p.q_begin, p.n_docs, p.rows_q, p.G, 128, slot, lane, tile));
-  const long vrows = (long)d.nq * p.G;
-  const long row0 = (long)tile * 128;
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, slot, lane, tile));
+  const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
 
-  // this lane's row
-  const long vr = row0 + wave * 32 + frow;
-  const long vrc = vr < vrows ? vr : vrows - 1;
-  const int qi = (int)(vrc / p.G), head = kvh * p.G + (int)(vrc - (long)qi * p.G);
+  // this lane's row; positions of the workgroup's and of this wave's rows
+  const int vr = row0 + wave * 32 + frow;
+  const int vrc = vr < vrows ? vr : vrows - 1;
+  const int qi = (int)((unsigned)vrc / (unsigned)p.G), head = kvh * p.G + vrc - qi * p.G;
   const int shift = d.nk - d.nq, pos = shift + qi;
   const size_t qrow = (size_t)d.q0 + qi;
-  // positions of the workgroup's and of this wave's rows
-  auto pos_of = [&](long r) { return shift + (int)((r < vrows ? r : vrows - 1) / p.G); };
+  auto pos_of = [&](int r) { return shift + (int)((unsigned)(r < vrows ? r : vrows - 1) / (unsigned)p.G); };
   const int wg0 = pos_of(row0), wg1 = pos_of(row0 + 127);
-  const int wv0 = pos_of(row0 + wave * 32), wv1 = pos_of(row0 + wave * 32 + 31);
+  const int wv0 = __builtin_amdgcn_readlane(pos, 0), wv1 = __builtin_amdgcn_readlane(pos, 31);
   const bool alive = row0 + wave * 32 < vrows;
 
   // the blocks to visit: those of the prefix, then those of the band
@@ -52,9 +52,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   if (bl < npre) bl = npre;
   const int nband = hi < 0 || hi / BK < bl ? 0 : hi / BK - bl + 1;
   const int nblk = npre + nband;
-  int it = (int)((long)sp * nblk / p.split);
-  const int it_end = (int)((long)(sp + 1) * nblk / p.split);
+  int it = p.split > 1 ? (int)((long)sp * nblk / p.split) : 0;
+  const int it_end = p.split > 1 ? (int)((long)(sp + 1) * nblk / p.split) : nblk;
 
+  const int cols = p.hd * T::ES / 16;
   const uint32_t ldkb = (uint32_t)(p.ld_k * T::ES), ldvb = (uint32_t)(p.ld_v * T::ES);
   const char* const kbase = reinterpret_cast<const char*>(p.k) + ((size_t)d.k0 * p.ld_k + (size_t)kvh * p.hd) * T::ES;
   const char* const vbase = reinterpret_cast<const char*>(p.v) + ((size_t)d.k0 * p.ld_v + (size_t)kvh * p.hd) * T::ES;
@@ -64,13 +65,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   auto block_of = [&](int i) { return i < npre ? i : i - npre + bl; };
   auto issue = [&](int i, int stage) {
     const int j0 = block_of(i) * BK;
-    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, p.hd, lds0 + stage * STAGE, wave, lane, vok);
-    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, p.hd, lds0 + stage * STAGE + TILE, wave, lane, vov);
+    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, cols, lds0 + stage * STAGE, wave, lane, vok);
+    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, cols, lds0 + stage * STAGE + TILE, wave, lane, vov);
   };
-  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, p.hd, tid, 256);
+  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, cols, tid, 256);
   if (it < it_end) issue(it, 0);
 
-  const int cols = p.hd * T::ES / 16;
   u32x4 qf[KS];
   {
     const char* qp = reinterpret_cast<const char*>(p.q) + (qrow * p.ld_q + (size_t)head * p.hd) * T::ES;
@@ -94,53 +94,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
+  const uint32_t kb = lds0 + TL::row_base(lane), vb = lds0 + TILE + TL::tr_base(lane);
   int stage = 0;
   for (; it < it_end; ++it) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (it + 1 < it_end) issue(it + 1, stage ^ 1);
     const int j0 = block_of(it) * BK;
-    const char* Ks = smem + stage * STAGE;
-    const char* Vs = Ks + TILE;
+    const uint32_t ka = kb + stage * STAGE, va = vb + stage * STAGE;
     stage ^= 1;
     const int cls = alive ? doc_class(p, wv0, wv1, j0, j0 + BK - 1, d.nk, d.pre) : 0;
     if (cls == 0) continue;
     f32x16 s[KT];
+    const int key_lane = j0 + 4 * half;
+    const float dist0 = (float)(pos - key_lane);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (2 * ks < cols) s[kt] = T::mma(TL::rowfrag(Ks, kt * 32 + frow, 2 * ks + half), qf[ks], s[kt]);
-    }
-    // scores (log2 domain), masks, block maximum
-    float mx = -INFINITY;
-    const int key_lane = j0 + 4 * half;
-    const float dist0 = (float)(pos - key_lane);
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+      for (int ks = 0; ks < KS; ++ks) s[kt] = T::mma(TL::row_read(ka, kt * 32, ks), qf[ks], s[kt]);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int off = kt * 32 + 8 * (r >> 2) + (r & 3);
         float rr;
-        s[kt][r] = doc_score<T, SHAPE>(p, s[kt][r], slope2, dist0 - (float)off, rr);
+        s[kt][r] = doc_score<T, SHAPE>(p, s[kt][r], slope2, dist0 - (float)(kt * 32 + 8 * (r >> 2) + (r & 3)), rr);
       }
+    }
     if (cls == 1) {
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = key_lane + kt * 32 + 8 * (r >> 2) + (r & 3);
-          const bool seen = key < d.pre || (key >= band.lo && key <= band.hi);
+          const bool seen = (key < d.pre) | ((key >= band.lo) & (key <= band.hi));
           s[kt][r] = seen ? s[kt][r] : -INFINITY;
         }
     }
+    float mx = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    mx = doc_half_max(mx);
     // The reference point moves only when a score passes it by 8 binary orders: p <= 2^8 stays far inside every type's range, and the
     // accumulators are rescaled a few times per row instead of once per block
     const bool up = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
@@ -152,40 +147,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
 #pragma unroll
       for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+        for (int r = 0; r < 16; ++r) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[i][r]) : "v"(alpha));  // (in place: as plain products the compiler copies all of o on every block)
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[kt][r] - m_use);
-        s[kt][r] = e;
-        l_run += e;
-      }
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
       for (int ss = 0; ss < 32 / T::STEP; ++ss) {
+#pragma unroll
+        for (int r = ss * T::STEP / 2; r < (ss + 1) * T::STEP / 2; ++r) {
+          const float e = __builtin_amdgcn_exp2f(s[kt][r] - m_use);
+          s[kt][r] = e;
+          l_run += e;
+        }
         const u32x4 pf = T::pack(s[kt], ss);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          if (dt * 32 < p.hd) o[dt] = T::mma(TL::trfrag(Vs, kt * 32 + T::STEP * ss, dt * 32, lane), pf, o[dt]);
+        for (int dt = 0; dt < DT; ++dt) o[dt] = T::mma(TL::tr_read(va, kt * 32 + T::STEP * ss, dt, lane), pf, o[dt]);
       }
   }
   __syncthreads();  // (the stages are idle: they become the waves' patches)
   if (!alive) return;
-  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  const float l = doc_half_sum(l_run);
   char* const patch = smem + wave * 32 * TL::RB;
   if (p.split == 1) {
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // (no key seen: zeros)
     if (p.lse != nullptr && half == 0 && vr < vrows)
       p.lse[(size_t)head * p.rows_q + qrow] = l == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(l)) * kLn2;
     doc_store_rows<T, HDP>(patch, o, inv, p.hd, lane, [&](int r) -> char* {
-      const long v = row0 + wave * 32 + r;
+      const int v = row0 + wave * 32 + r;
       if (v >= vrows) return nullptr;
-      const int i = (int)(v / p.G);
-      return reinterpret_cast<char*>(p.out) + (((size_t)d.q0 + i) * p.ld_o + (size_t)(kvh * p.G + (int)(v - (long)i * p.G)) * p.hd) * T::ES;
+      const int i = (int)((unsigned)v / (unsigned)p.G);
+      return reinterpret_cast<char*>(p.out) + (((size_t)d.q0 + i) * p.ld_o + (size_t)(kvh * p.G + v - i * p.G) * p.hd) * T::ES;
     });
   } else {
     if (vr < vrows) {
@@ -234,10 +226,10 @@ template <typename T> __global__ __launch_bounds__(256) void doc_join_kernel(Doc
   if (c == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <typename T, int HDP, int SHAPE> int run_doc_attn(const DocAttnP& p, hipStream_t st) {
+template <typename T, int HDP, int KS, int SHAPE> int run_doc_attn(const DocAttnP& p, hipStream_t st) {
   constexpr int lds = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * DocTile<T, HDP>::RB;
   constexpr int bytes = lds > patch ? lds : patch;
-  const auto kernel = doc_attn_kernel<T, HDP, SHAPE>;
+  const auto kernel = doc_attn_kernel<T, HDP, KS, SHAPE>;
   if (bytes > 64 * 1024) OSUD_BIG_LDS_ONCE(kernel);
   kernel<<<dim3((unsigned)(p.slots * p.kv_heads * p.split)), 256, bytes, st>>>(p);
   OSUD_HIP(hipGetLastError());
@@ -248,26 +240,48 @@ template <typename T, int HDP, int SHAPE> int run_doc_attn(const DocAttnP& p, hi
   }
   return OSUD_OK;
 }
-template <typename T, int HDP> int run_doc_attn_shape(const DocAttnP& p, hipStream_t st) {
+template <typename T, int HDP, int KS> int run_doc_attn_shape(const DocAttnP& p, hipStream_t st) {
   switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
-    case 0: return run_doc_attn<T, HDP, 0>(p, st);
-    case kShapeCap: return run_doc_attn<T, HDP, kShapeCap>(p, st);
-    case kShapeSlope: return run_doc_attn<T, HDP, kShapeSlope>(p, st);
-    default: return run_doc_attn<T, HDP, kShapeCap | kShapeSlope>(p, st);
+    case 0: return run_doc_attn<T, HDP, KS, 0>(p, st);
+    case kShapeCap: return run_doc_attn<T, HDP, KS, kShapeCap>(p, st);
+    case kShapeSlope: return run_doc_attn<T, HDP, KS, kShapeSlope>(p, st);
+    default: return run_doc_attn<T, HDP, KS, kShapeCap | kShapeSlope>(p, st);
   }
 }
+// widths of 64, 96 and 128 columns; 65 .. 80 columns skip the contraction steps of the last sixteen pad columns
 template <typename T> int run_doc_attn_hd(const DocAttnP& p, hipStream_t st) {
-  if (p.hd <= 64) return run_doc_attn_shape<T, 64>(p, st);
-  if (p.hd <= 96) return run_doc_attn_shape<T, 96>(p, st);
-  return run_doc_attn_shape<T, 128>(p, st);
+  constexpr int N = T::ES == 2 ? 16 : 8;
+  if (p.hd <= 64) return run_doc_attn_shape<T, 64, 64 / N>(p, st);
+  if (p.hd <= 80) return run_doc_attn_shape<T, 96, 80 / N>(p, st);
+  if (p.hd <= 96) return run_doc_attn_shape<T, 96, 96 / N>(p, st);
+  return run_doc_attn_shape<T, 128, 128 / N>(p, st);
+}
+
+// Parts of the key axis: few tiles (no more than one per CU) of long documents leave most of the chip idle; up to four workgroups per CU then, each
+// with at least 512 keys (a part leaves and re-reads 128 rows x head_dim floats: as much as 128 keys).
+int doc_split(const DocAttnP& p, int max_k) {
+  const int cus = device_cus(), tiles = p.slots * p.kv_heads;
+  const long keys = max_k > 0 ? max_k : p.rows_k / (p.n_docs > 0 ? p.n_docs : 1);
+  if (tiles <= 0 || tiles > cus) return 1;
+  long n = 4L * cus / tiles;
+  if (n > keys / 512) n = keys / 512;
+  if (n > 64) n = 64;
+  return n < 1 ? 1 : (int)n;
 }
 
 }  // namespace
 
-size_t doc_attn_ws(const DocAttnP&, int, int) { return 0; }
+size_t doc_attn_ws(const DocAttnP& p, int, int max_k) {
+  const size_t n = doc_split(p, max_k);
+  return n > 1 ? n * p.rows_q * p.heads * (p.hd + 2) : 0;
+}
 
 int launch_doc_attn(int prec, DocAttnP& p, int max_k, size_t ws_floats, hipStream_t st) {
-  p.split = 1;
+  p.split = doc_split(p, max_k);
+  const size_t part = (size_t)p.rows_q * p.heads * (p.hd + 2);
+  if (p.split > 1 && (size_t)p.split * part > ws_floats) p.split = ws_floats / part < 2 ? 1 : (int)(ws_floats / part);
+  p.ws_ml = p.ws_o;
+  if (p.split > 1) p.ws_ml += (size_t)p.split * p.rows_q * p.heads * p.hd;
   if (prec == OSUD_PREC_BF16) return run_doc_attn_hd<DocBf16>(p, st);
   if (prec == OSUD_PREC_F16) return run_doc_attn_hd<DocF16>(p, st);
   return run_doc_attn_hd<DocF32>(p, st);

@@ -11,20 +11,23 @@
 namespace osud {
 namespace {
 
-// p and ds of one pair.  `v`: q.k;  lse2 = lse * log2(e)
+// p of one pair, and (cap) the factor 1 - tanh^2.  `qk`: q.k;  lse2 = lse * log2(e)
 template <typename T, int SHAPE>
-__device__ __forceinline__ void doc_pair(const DocAttnP& p, float qk, float dp, float slope2, float distance, float lse2, float delta, bool seen, float& prob, float& ds) {
+__device__ __forceinline__ float doc_weight(const DocAttnP& p, float qk, float slope2, float distance, float lse2, float& dsc) {
   float r = 0.f;
   const float v = doc_score<T, SHAPE>(p, qk, slope2, distance, r);
-  prob = seen ? __builtin_amdgcn_exp2f(v - lse2) : 0.f;
-  ds = prob * (dp - delta);
-  if constexpr ((SHAPE & kShapeCap) != 0) ds *= 4.0f * r * (1.0f - r);
+  dsc = (SHAPE & kShapeCap) != 0 ? 4.0f * r * (1.0f - r) : 1.0f;
+  return __builtin_amdgcn_exp2f(v - lse2);
+}
+template <int SHAPE> __device__ __forceinline__ float doc_ds(float prob, float dp, float delta, float dsc) {
+  const float ds = prob * (dp - delta);
+  return (SHAPE & kShapeCap) != 0 ? ds * dsc : ds;
 }
 
-template <typename T, int HDP, int SHAPE>
+template <typename T, int HDP, int KS, int SHAPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 && T::ES == 4 ? 1 : 2))) void doc_attn_dq_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
-  constexpr int BK = T::BK, KT = BK / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
   constexpr int TILE = ST::BYTES, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -35,18 +38,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   const int u = doc_unit(blockIdx.x, gridDim.x);
   const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);
   int tile;
-  const DocRange d = doc_range(p, doc_find(p.q_begin, p.n_docs, p.rows_q, p.G, 128, slot, lane, tile));
-  const long vrows = (long)d.nq * p.G;
-  const long row0 = (long)tile * 128;
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, slot, lane, tile));
+  const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
-  const long vr = row0 + wave * 32 + frow;
-  const long vrc = vr < vrows ? vr : vrows - 1;
-  const int qi = (int)(vrc / p.G), head = kvh * p.G + (int)(vrc - (long)qi * p.G);
+  const int vr = row0 + wave * 32 + frow;
+  const int vrc = vr < vrows ? vr : vrows - 1;
+  const int qi = (int)((unsigned)vrc / (unsigned)p.G), head = kvh * p.G + vrc - qi * p.G;
   const int shift = d.nk - d.nq, pos = shift + qi;
   const size_t qrow = (size_t)d.q0 + qi;
-  auto pos_of = [&](long r) { return shift + (int)((r < vrows ? r : vrows - 1) / p.G); };
+  auto pos_of = [&](int r) { return shift + (int)((unsigned)(r < vrows ? r : vrows - 1) / (unsigned)p.G); };
   const int wg0 = pos_of(row0), wg1 = pos_of(row0 + 127);
-  const int wv0 = pos_of(row0 + wave * 32), wv1 = pos_of(row0 + wave * 32 + 31);
+  const int wv0 = __builtin_amdgcn_readlane(pos, 0), wv1 = __builtin_amdgcn_readlane(pos, 31);
   const bool alive = row0 + wave * 32 < vrows;
 
   const int npre = (d.pre + BK - 1) / BK;
@@ -55,6 +57,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   if (bl < npre) bl = npre;
   const int nblk = npre + (hi < 0 || hi / BK < bl ? 0 : hi / BK - bl + 1);
 
+  const int cols = p.hd * T::ES / 16;
   const uint32_t ldkb = (uint32_t)(p.ld_k * T::ES), ldvb = (uint32_t)(p.ld_v * T::ES);
   const char* const kbase = reinterpret_cast<const char*>(p.k) + ((size_t)d.k0 * p.ld_k + (size_t)kvh * p.hd) * T::ES;
   const char* const vbase = reinterpret_cast<const char*>(p.v) + ((size_t)d.k0 * p.ld_v + (size_t)kvh * p.hd) * T::ES;
@@ -64,13 +67,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   auto block_of = [&](int i) { return i < npre ? i : i - npre + bl; };
   auto issue = [&](int i, int stage) {
     const int j0 = block_of(i) * BK;
-    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, p.hd, lds0 + stage * STAGE, wave, lane, vok);
-    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, p.hd, lds0 + stage * STAGE + TILE, wave, lane, vov);
+    ST::load(kbase + (size_t)j0 * ldkb, d.nk - j0, ldkb, cols, lds0 + stage * STAGE, wave, lane, vok);
+    ST::load(vbase + (size_t)j0 * ldvb, d.nk - j0, ldvb, cols, lds0 + stage * STAGE + TILE, wave, lane, vov);
   };
-  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, p.hd, tid, 256);
+  for (int i = 0; i < 4; ++i) ST::clear_pads(smem + i * TILE, cols, tid, 256);
   if (nblk > 0) issue(0, 0);
 
-  const int cols = p.hd * T::ES / 16;
   u32x4 qf[KS], gf[KS];
   float delta = 0.f;
   {
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
       }
     }
   }
-  delta += __shfl_xor(delta, 32, 64);
+  delta = doc_half_sum(delta);
   const size_t at = (size_t)head * p.rows_q + qrow, n_at = (size_t)p.heads * p.rows_q;
   const float lse = p.lse[at];
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key seen: every p is 0)
@@ -109,14 +111,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
+  const uint32_t kb = lds0 + TL::row_base(lane), tb = lds0 + TL::tr_base(lane);
   for (int it = 0; it < nblk; ++it) {
     const int stage = it & 1;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (it + 1 < nblk) issue(it + 1, stage ^ 1);
     const int j0 = block_of(it) * BK;
-    const char* Ks = smem + stage * STAGE;
-    const char* Vs = Ks + TILE;
+    const uint32_t ka = kb + stage * STAGE, va = ka + TILE, ta = tb + stage * STAGE;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       const int cls = alive ? doc_class(p, wv0, wv1, j0 + kt * 32, j0 + kt * 32 + 31, d.nk, d.pre) : 0;
@@ -125,46 +127,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (2 * ks < cols) {
-          s = T::mma(TL::rowfrag(Ks, kt * 32 + frow, 2 * ks + half), qf[ks], s);
-          dp = T::mma(TL::rowfrag(Vs, kt * 32 + frow, 2 * ks + half), gf[ks], dp);
-        }
+      for (int ks = 0; ks < KS; ++ks) s = T::mma(TL::row_read(ka, kt * 32, ks), qf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = T::mma(TL::row_read(va, kt * 32, ks), gf[ks], dp);
       const int key_lane = j0 + kt * 32 + 4 * half;
       const float dist0 = (float)(pos - key_lane);
+      float dsc[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int off = 8 * (r >> 2) + (r & 3), key = key_lane + off;
-        const bool seen = cls == 2 || key < d.pre || (key >= band.lo && key <= band.hi);
-        float prob, ds;
-        doc_pair<T, SHAPE>(p, s[r], dp[r], slope2, dist0 - (float)off, lse2, delta, seen, prob, ds);
-        s[r] = ds;
+      for (int r = 0; r < 16; ++r) s[r] = doc_weight<T, SHAPE>(p, s[r], slope2, dist0 - (float)(8 * (r >> 2) + (r & 3)), lse2, dsc[r]);
+      if (cls == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key_lane + 8 * (r >> 2) + (r & 3);
+          const bool seen = (key < d.pre) | ((key >= band.lo) & (key <= band.hi));
+          s[r] = seen ? s[r] : 0.f;
+        }
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = doc_ds<SHAPE>(s[r], dp[r], delta, dsc[r]);
 #pragma unroll
       for (int ss = 0; ss < 32 / T::STEP; ++ss) {
         const u32x4 f = T::pack(s, ss);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          if (dt * 32 < p.hd) dq[dt] = T::mma(TL::trfrag(Ks, kt * 32 + T::STEP * ss, dt * 32, lane), f, dq[dt]);
+        for (int dt = 0; dt < DT; ++dt) dq[dt] = T::mma(TL::tr_read(ta, kt * 32 + T::STEP * ss, dt, lane), f, dq[dt]);
       }
     }
   }
   __syncthreads();
   if (!alive) return;
   doc_store_rows<T, HDP>(smem + wave * 32 * TL::RB, dq, p.scale, p.hd, lane, [&](int r) -> char* {
-    const long v = row0 + wave * 32 + r;
+    const int v = row0 + wave * 32 + r;
     if (v >= vrows) return nullptr;
-    const int i = (int)(v / p.G);
-    return reinterpret_cast<char*>(p.dq) + (((size_t)d.q0 + i) * p.ld_dq + (size_t)(kvh * p.G + (int)(v - (long)i * p.G)) * p.hd) * T::ES;
+    const int i = (int)((unsigned)v / (unsigned)p.G);
+    return reinterpret_cast<char*>(p.dq) + (((size_t)d.q0 + i) * p.ld_dq + (size_t)(kvh * p.G + v - i * p.G) * p.hd) * T::ES;
   });
 }
 
 // One workgroup = 128 keys of one document and key head (a wave owns 32: lane = key); the shared heads one after the other, for each the
 // query blocks that see the keys.  With a split (few key tiles), part `sp` takes its share of the (head, block) list and leaves fp32 sums.
-template <typename T, int HDP, int SHAPE>
+template <typename T, int HDP, int KS, int SHAPE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 || T::ES == 4 ? 1 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
-  constexpr int BQ = T::BK, QT = BQ / 32, KS = HDP * T::ES / 32, DT = HDP / 32;
+  constexpr int BQ = T::BK, QT = BQ / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BQ, 4>;
   constexpr int TILE = ST::BYTES, STAGE = 2 * TILE + 2 * BQ * 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -173,11 +177,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   const int frow = lane & 31, half = lane >> 5;
 
   int u = doc_unit(blockIdx.x, gridDim.x);
-  const int sp = u % p.split;
-  u /= p.split;
+  const int sp = p.split > 1 ? u % p.split : 0;
+  if (p.split > 1) u /= p.split;
   const int kvh = u / p.slots, slot = u - kvh * p.slots;
   int tile;
-  const DocRange d = doc_range(p, doc_find(p.k_begin, p.n_docs, p.rows_k, 1, 128, slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.k_begin, p.n_docs, p.rows_k, 1, slot, lane, tile));
   const int j0 = tile * 128;
   if (tile < 0 || j0 >= d.nk) return;
   const int jw = j0 + wave * 32;  // this wave's first key
@@ -194,9 +198,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   }
   const int b0 = i_lo / BQ, nb = i_hi < i_lo ? 0 : i_hi / BQ - b0 + 1;
   const int total = nb * p.G;
-  int it = (int)((long)sp * total / p.split);
-  const int it_end = (int)((long)(sp + 1) * total / p.split);
+  int it = p.split > 1 ? (int)((long)sp * total / p.split) : 0;
+  const int it_end = p.split > 1 ? (int)((long)(sp + 1) * total / p.split) : total;
 
+  const int cols = p.hd * T::ES / 16;
   const uint32_t ldqb = (uint32_t)(p.ld_q * T::ES), ldgb = (uint32_t)(p.ld_do * T::ES);
   uint32_t voq[ST::PER], vog[ST::PER];
   ST::offsets(wave, lane, ldqb, voq);
@@ -206,8 +211,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
     const int g = i / nb, i0 = (b0 + i - g * nb) * BQ, head = kvh * p.G + g;
     const size_t row = (size_t)d.q0 + i0;
     const uint32_t lds = lds0 + stage * STAGE;
-    ST::load(reinterpret_cast<const char*>(p.q) + (row * p.ld_q + (size_t)head * p.hd) * T::ES, d.nq - i0, ldqb, p.hd, lds, wave, lane, voq);
-    ST::load(reinterpret_cast<const char*>(p.d_o) + (row * p.ld_do + (size_t)head * p.hd) * T::ES, d.nq - i0, ldgb, p.hd, lds + TILE, wave, lane, vog);
+    ST::load(reinterpret_cast<const char*>(p.q) + (row * p.ld_q + (size_t)head * p.hd) * T::ES, d.nq - i0, ldqb, cols, lds, wave, lane, voq);
+    ST::load(reinterpret_cast<const char*>(p.d_o) + (row * p.ld_do + (size_t)head * p.hd) * T::ES, d.nq - i0, ldgb, cols, lds + TILE, wave, lane, vog);
     if (wave < 2 && lane < BQ) {  // wave 0: delta, wave 1: lse2 of the block's rows
       const float* src = p.delta + (wave == 1 ? n_at : 0) + (size_t)head * p.rows_q + row;
       const uint32_t off = (uint32_t)(i0 + lane < d.nq ? lane : d.nq - 1 - i0) * 4u;
@@ -215,12 +220,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
     }
   };
   for (int i = 0; i < 2; ++i) {
-    ST::clear_pads(smem + i * STAGE, p.hd, tid, 256);
-    ST::clear_pads(smem + i * STAGE + TILE, p.hd, tid, 256);
+    ST::clear_pads(smem + i * STAGE, cols, tid, 256);
+    ST::clear_pads(smem + i * STAGE + TILE, cols, tid, 256);
   }
   if (it < it_end) issue(it, 0);
 
-  const int cols = p.hd * T::ES / 16;
   u32x4 kf[KS], vf[KS];
   {
     const char* kp = reinterpret_cast<const char*>(p.k) + (((size_t)d.k0 + keyc) * p.ld_k + (size_t)kvh * p.hd) * T::ES;
@@ -244,6 +248,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+  const uint32_t qb = lds0 + TL::row_base(lane), tb = lds0 + TL::tr_base(lane);
+  // queries whose band holds this lane's key
+  const int band_lo = p.right < 0 ? 0 : key - p.right - shift, band_hi = p.left < 0 ? d.nq : key + p.left - shift;
   int stage = 0;
   for (; it < it_end; ++it) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -252,9 +259,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
     const int g = it / nb, i0 = (b0 + it - g * nb) * BQ;
     float slope2 = 0.f;
     if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[kvh * p.G + g] * kLog2e;
-    const char* Qs = smem + stage * STAGE;
-    const char* Gs = Qs + TILE;
-    const float* rows = reinterpret_cast<const float*>(Qs + 2 * TILE);  // delta [BQ], lse2 [BQ]
+    const uint32_t qa = qb + stage * STAGE, ga = qa + TILE, tq = tb + stage * STAGE, tg = tq + TILE;
+    const float* rows = reinterpret_cast<const float*>(smem + stage * STAGE + 2 * TILE);  // delta [BQ], lse2 [BQ]
     stage ^= 1;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -267,40 +273,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if (2 * ks < cols) {
-          s = T::mma(TL::rowfrag(Qs, qt * 32 + frow, 2 * ks + half), kf[ks], s);
-          dp = T::mma(TL::rowfrag(Gs, qt * 32 + frow, 2 * ks + half), vf[ks], dp);
-        }
+      for (int ks = 0; ks < KS; ++ks) s = T::mma(TL::row_read(qa, qt * 32, ks), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = T::mma(TL::row_read(ga, qt * 32, ks), vf[ks], dp);
       const int qi0 = i + 4 * half;
       const float dist0 = (float)(shift + qi0 - key);
+      float dsc[16];
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[4 * q4 + e] = doc_weight<T, SHAPE>(p, s[4 * q4 + e], slope2, dist0 + (float)(8 * q4 + e), ls[e], dsc[4 * q4 + e]);
+      }
+      if (cls == 1) {
+        const int none = key < d.nk ? d.nq : 0;  // queries below this one exist, for a key that exists
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int qi = qi0 + 8 * (r >> 2) + (r & 3);
+          const bool seen = (qi < none) & ((key < d.pre) | ((qi >= band_lo) & (qi <= band_hi)));
+          s[r] = seen ? s[r] : 0.f;
+        }
+      }
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const f32x4 de = *reinterpret_cast<const f32x4*>(rows + qt * 32 + 8 * q4 + 4 * half);
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int off = 8 * q4 + e, pos = shift + qi0 + off;
-          bool seen = true;
-          if (cls == 1) {
-            const bool band = (p.left < 0 || key >= pos - p.left) && (p.right < 0 || key <= pos + p.right);
-            seen = qi0 + off < d.nq && key < d.nk && (band || key < d.pre);
-          }
-          float prob, ds;
-          doc_pair<T, SHAPE>(p, s[4 * q4 + e], dp[4 * q4 + e], slope2, dist0 + (float)off, ls[e], de[e], seen, prob, ds);
-          s[4 * q4 + e] = prob;
-          dp[4 * q4 + e] = ds;
-        }
+        for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = doc_ds<SHAPE>(s[4 * q4 + e], dp[4 * q4 + e], de[e], dsc[4 * q4 + e]);
       }
 #pragma unroll
       for (int ss = 0; ss < 32 / T::STEP; ++ss) {
         const u32x4 pf = T::pack(s, ss), df = T::pack(dp, ss);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          if (dt * 32 < p.hd) {
-            dv[dt] = T::mma(TL::trfrag(Gs, qt * 32 + T::STEP * ss, dt * 32, lane), pf, dv[dt]);
-            dk[dt] = T::mma(TL::trfrag(Qs, qt * 32 + T::STEP * ss, dt * 32, lane), df, dk[dt]);
-          }
+        for (int dt = 0; dt < DT; ++dt) dv[dt] = T::mma(TL::tr_read(tg, qt * 32 + T::STEP * ss, dt, lane), pf, dv[dt]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dk[dt] = T::mma(TL::tr_read(tq, qt * 32 + T::STEP * ss, dt, lane), df, dk[dt]);
       }
     }
   }
@@ -357,13 +364,13 @@ template <typename T> __global__ __launch_bounds__(256) void doc_dkv_join_kernel
   store8(reinterpret_cast<typename T::E*>(is_k ? p.dk : p.dv) + row * (is_k ? p.ld_dk : p.ld_dv) + (size_t)kvh * p.hd + c, acc);
 }
 
-template <typename T, int HDP, int SHAPE> int run_doc_bwd(const DocAttnP& p0, hipStream_t st) {
+template <typename T, int HDP, int KS, int SHAPE> int run_doc_bwd(const DocAttnP& p0, hipStream_t st) {
   using TL = DocTile<T, HDP>;
   DocAttnP p = p0;
   constexpr int tiles = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * TL::RB;
   constexpr int bytes_q = tiles > patch ? tiles : patch, bytes_k = (tiles > patch ? tiles : patch) + 4 * T::BK * 4;
-  const auto kq = doc_attn_dq_kernel<T, HDP, SHAPE>;
-  const auto kk = doc_attn_dkv_kernel<T, HDP, SHAPE>;
+  const auto kq = doc_attn_dq_kernel<T, HDP, KS, SHAPE>;
+  const auto kk = doc_attn_dkv_kernel<T, HDP, KS, SHAPE>;
   if (bytes_q > 64 * 1024) OSUD_BIG_LDS_ONCE(kq);
   if (bytes_k > 64 * 1024) OSUD_BIG_LDS_ONCE(kk);
   p.slots = (int)((long)p.rows_q * p.G / 128) + p.n_docs;
@@ -379,26 +386,46 @@ template <typename T, int HDP, int SHAPE> int run_doc_bwd(const DocAttnP& p0, hi
   }
   return OSUD_OK;
 }
-template <typename T, int HDP> int run_doc_bwd_shape(const DocAttnP& p, hipStream_t st) {
+template <typename T, int HDP, int KS> int run_doc_bwd_shape(const DocAttnP& p, hipStream_t st) {
   switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
-    case 0: return run_doc_bwd<T, HDP, 0>(p, st);
-    case kShapeCap: return run_doc_bwd<T, HDP, kShapeCap>(p, st);
-    case kShapeSlope: return run_doc_bwd<T, HDP, kShapeSlope>(p, st);
-    default: return run_doc_bwd<T, HDP, kShapeCap | kShapeSlope>(p, st);
+    case 0: return run_doc_bwd<T, HDP, KS, 0>(p, st);
+    case kShapeCap: return run_doc_bwd<T, HDP, KS, kShapeCap>(p, st);
+    case kShapeSlope: return run_doc_bwd<T, HDP, KS, kShapeSlope>(p, st);
+    default: return run_doc_bwd<T, HDP, KS, kShapeCap | kShapeSlope>(p, st);
   }
 }
 template <typename T> int run_doc_bwd_hd(const DocAttnP& p, hipStream_t st) {
-  if (p.hd <= 64) return run_doc_bwd_shape<T, 64>(p, st);
-  if (p.hd <= 96) return run_doc_bwd_shape<T, 96>(p, st);
-  return run_doc_bwd_shape<T, 128>(p, st);
+  constexpr int N = T::ES == 2 ? 16 : 8;
+  if (p.hd <= 64) return run_doc_bwd_shape<T, 64, 64 / N>(p, st);
+  if (p.hd <= 80) return run_doc_bwd_shape<T, 96, 80 / N>(p, st);
+  if (p.hd <= 96) return run_doc_bwd_shape<T, 96, 96 / N>(p, st);
+  return run_doc_bwd_shape<T, 128, 128 / N>(p, st);
+}
+
+// Parts of the query axis of the key kernel: as in the forward pass, where its tiles do not give every CU four workgroups (one wave per SIMD
+// at 128 columns: the parts also even out a causal mask); at least 512 query rows per part, at most 16 parts.
+int doc_bwd_split(const DocAttnP& p, int max_q) {
+  const int cus = device_cus(), tiles = (p.rows_k / 128 + p.n_docs) * p.kv_heads;
+  const long rows = (long)(max_q > 0 ? max_q : p.rows_q / (p.n_docs > 0 ? p.n_docs : 1)) * p.G;
+  if (tiles <= 0 || tiles > 2 * cus) return 1;
+  long n = 4L * cus / tiles;
+  if (n > rows / 512) n = rows / 512;
+  if (n > 16) n = 16;
+  return n < 1 ? 1 : (int)n;
 }
 
 }  // namespace
 
-size_t doc_attn_bwd_ws(const DocAttnP& p, int) { return 2 * (size_t)p.heads * p.rows_q; }
+size_t doc_attn_bwd_ws(const DocAttnP& p, int max_q) {
+  const size_t n = doc_bwd_split(p, max_q), rows = 2 * (size_t)p.heads * p.rows_q;
+  return (rows + 3) / 4 * 4 + (n > 1 ? n * p.rows_k * p.kv_heads * 2 * p.hd : 0);
+}
 
 int launch_doc_attn_bwd(int prec, DocAttnP& p, int max_q, size_t ws_floats, hipStream_t st) {
-  p.split = 1;
+  const size_t rows = (2 * (size_t)p.heads * p.rows_q + 3) / 4 * 4, part = (size_t)p.rows_k * p.kv_heads * 2 * p.hd;
+  p.split = doc_bwd_split(p, max_q);
+  if (p.split > 1 && rows + p.split * part > ws_floats) p.split = ws_floats < rows + 2 * part ? 1 : (int)((ws_floats - rows) / part);
+  p.ws_o = p.delta + rows;
   return prec == OSUD_PREC_BF16 ? run_doc_bwd_hd<DocBf16>(p, st) : run_doc_bwd_hd<DocF32>(p, st);
 }
 

@@ -56,6 +56,7 @@ int doc_params(const char* who, const osud_doc_attention* a, bool back, DocAttnP
                  "%s: a row stride is shorter than its heads or not a multiple of 16 bytes", who);
   const int G = a->heads / a->kv_heads;
   const int64_t tiles = ((int64_t)a->rows_q * G / 128 + a->n_docs) * a->kv_heads, ktiles = ((int64_t)a->rows_k / 128 + a->n_docs) * a->kv_heads;
+  OSUD_CHECK_ARG((int64_t)a->rows_q * G < (1L << 31) - 128, "%s: %d query rows of %d shared heads", who, a->rows_q, G);
   OSUD_CHECK_ARG(tiles < (1 << 24) && ktiles < (1 << 24), "%s: too many tiles for one launch", who);
   DocAttnP z = {};
   z.ld_q = a->ld_q; z.ld_k = a->ld_k; z.ld_v = a->ld_v; z.ld_o = a->ld_out;
