@@ -181,9 +181,8 @@ template <int bm> __device__ __forceinline__ int doc_find(const int32_t* begin, 
   auto start = [&](int d) { return (int)((unsigned)(doc_clamp(begin[d], 0, rows) * m) / (unsigned)bm) + d; };  // (rows * m < 2^31)
   int lo = 0, len = n_docs;
   while (len > 1) {
-    const int step = (len + 63) >> 6, d = lo + lane * step;
-    const bool in = lane * step < len && start(d) <= slot;
-    int n = __popcll(__ballot(in));
+    const int step = (len + 63) >> 6, i = lane * step;
+    int n = __popcll(__ballot(i < len && start(lo + (i < len ? i : 0)) <= slot));
     n = n < 1 ? 1 : n;
     const int skip = (n - 1) * step;
     lo += skip;

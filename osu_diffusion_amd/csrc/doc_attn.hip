@@ -15,7 +15,7 @@ namespace osud {
 namespace {
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? ((SHAPE & kShapeSlope) != 0 ? 3 : 4) : HDP == 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
@@ -194,36 +194,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   }
 }
 
-// joins the parts of a split: one thread per (row, head, 8 columns), parts in order
+// joins the parts of a split (at most 64): one wave per (row, head); lane s takes part s's weight, then every lane 2 columns of all parts, in order
 template <typename T> __global__ __launch_bounds__(256) void doc_join_kernel(DocAttnP p) {
-  const int cpr = p.hd / 8;
-  const size_t n = (size_t)p.rows_q * p.heads;
-  const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t at = idx / cpr;
-  const int c = (int)(idx - at * cpr) * 8;
+  const int lane = threadIdx.x & 63;
+  const size_t n = (size_t)p.rows_q * p.heads, at = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (at >= n) return;
-  const size_t row = at / p.heads;
-  const int head = (int)(at - row * p.heads);
-  const int last = doc_clamp(p.q_begin[p.n_docs], 0, p.rows_q);
-  if ((long)row >= last || (long)row < doc_clamp(p.q_begin[0], 0, p.rows_q)) return;  // (rows of no document: nothing was written for them)
-  float m = -INFINITY;
-  for (int s = 0; s < p.split; ++s) m = fmaxf(m, p.ws_ml[2 * (s * n + at)]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[8] = {};
-  for (int s = 0; s < p.split; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (s * n + at));
-    const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mu);
-    l = fmaf(ml.y, w, l);
-    float v[8];
-    load8(p.ws_o + (s * n + at) * p.hd + c, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+  const int row = (int)(at / p.heads), head = (int)(at - (size_t)row * p.heads);
+  if (row >= doc_clamp(p.q_begin[p.n_docs], 0, p.rows_q) || row < doc_clamp(p.q_begin[0], 0, p.rows_q)) return;  // (no document's: nothing was written)
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < p.split) ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (lane * n + at));
+  const float m = wave_max(ml.x), mu = m == -INFINITY ? 0.f : m;
+  const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mu);
+  const float l = wave_sum(ml.y * w);
+  float a0 = 0.f, a1 = 0.f;
+  const float* src = p.ws_o + at * p.hd + 2 * lane;
+  if (2 * lane < p.hd) {
+#pragma unroll 8
+    for (int s = 0; s < p.split; ++s) {
+      const float2 v = *reinterpret_cast<const float2*>(src + s * n * p.hd);
+      const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+      a0 = fmaf(v.x, ws, a0);
+      a1 = fmaf(v.y, ws, a1);
+    }
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    store2(reinterpret_cast<typename T::E*>(p.out) + (size_t)row * p.ld_o + (size_t)head * p.hd + 2 * lane, a0 * inv, a1 * inv);
   }
-  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] *= inv;
-  store8(reinterpret_cast<typename T::E*>(p.out) + row * p.ld_o + (size_t)head * p.hd + c, acc);
-  if (c == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (lane == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 template <typename T, int HDP, int KS, int SHAPE> int run_doc_attn(const DocAttnP& p, hipStream_t st) {
@@ -234,8 +230,7 @@ template <typename T, int HDP, int KS, int SHAPE> int run_doc_attn(const DocAttn
   kernel<<<dim3((unsigned)(p.slots * p.kv_heads * p.split)), 256, bytes, st>>>(p);
   OSUD_HIP(hipGetLastError());
   if (p.split > 1) {
-    const size_t items = (size_t)p.rows_q * p.heads * (p.hd / 8);
-    doc_join_kernel<T><<<dim3((unsigned)((items + 255) / 256)), 256, 0, st>>>(p);
+    doc_join_kernel<T><<<dim3((unsigned)(((size_t)p.rows_q * p.heads + 3) / 4)), 256, 0, st>>>(p);
     OSUD_HIP(hipGetLastError());
   }
   return OSUD_OK;

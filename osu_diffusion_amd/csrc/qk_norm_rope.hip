@@ -8,6 +8,8 @@
 // R + i; interleaved: 2 W neighbouring columns), so the rotation needs no exchange and the norm a few lane shuffles.  A workgroup takes
 // TPB rows: their angles first, one per lane, into LDS -- each serves all heads of its row.  position * f / 2 pi is taken in 64 bits and
 // reduced to a fraction of a turn there: at 10^6 positions a product in 32 bits is off by 0.06 radians.
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -41,51 +43,88 @@ __device__ __forceinline__ void rope_angles(const RopeP& p, long t0, int n, floa
   }
 }
 
-// one lane's two chunks of a head: columns ca .. ca + W - 1 and cb .. cb + W - 1
-template <int W> struct RopeLane {
+// one lane's two chunks of a head: columns ca .. ca + W - 1 and cb .. cb + W - 1 (INTER: cb = ca + W)
+template <int W, bool INTER> struct RopeLane {
   int ca, cb, pair;
   bool a, b, turn;
   __device__ __forceinline__ RopeLane(const RopeP& p, int l) {
     const int R = p.rot / 2, np = R / W;
     turn = l < np;
-    pair = l * W;
-    if (turn) {
-      ca = p.interleaved ? 2 * pair : pair;
-      cb = p.interleaved ? 2 * pair + W : R + pair;
-      a = b = true;
-    } else {
-      ca = p.rot + 2 * W * (l - np);
+    pair = turn ? l * W : 0;
+    if (INTER || !turn) {
+      ca = (INTER ? 0 : p.rot) + 2 * W * (l - (INTER ? 0 : np));
       cb = ca + W;
-      a = ca < p.hd;
-      b = cb < p.hd;
+    } else {
+      ca = pair;
+      cb = R + pair;
     }
+    a = ca < p.hd;
+    b = cb < p.hd;
   }
 };
 // (x[0 .. 2 W - 1] = chunk a, chunk b)  the rotation, or its transpose
-template <int W, bool BACK> __device__ __forceinline__ void rope_turn(const float2* cs, bool interleaved, float (&x)[2 * W]) {
+template <int W, bool INTER, bool BACK> __device__ __forceinline__ void rope_turn(const float2* cs, float (&x)[2 * W]) {
 #pragma unroll
   for (int i = 0; i < W; ++i) {
+    const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : W + i;
     float2 t = cs[i];
     if (BACK) t.y = -t.y;
-    const float a0 = x[2 * i], b0 = x[2 * i + 1], a1 = x[i], b1 = x[W + i];
-    // (both layouts, selected by a uniform value; the half layout writes below)
-    if (interleaved) {
-      x[2 * i] = a0 * t.x - b0 * t.y;
-      x[2 * i + 1] = a0 * t.y + b0 * t.x;
-    } else {
-      x[i] = a1 * t.x - b1 * t.y;
-      x[W + i] = a1 * t.y + b1 * t.x;
+    const float a = x[ia], b = x[ib];
+    x[ia] = a * t.x - b * t.y;
+    x[ib] = a * t.y + b * t.x;
+  }
+}
+// both chunks of a head (INTER: they are one)
+template <int W, bool INTER, typename E> __device__ __forceinline__ void load_lane(const E* p, const RopeLane<W, INTER>& ln, float (&x)[2 * W]) {
+  if constexpr (INTER && W <= 4) {
+    float v[2 * W] = {};
+    if (ln.a) load_chunk<2 * W>(p + ln.ca, v);
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) x[i] = v[i];
+  } else {
+    float a[W] = {}, b[W] = {};
+    if (ln.a) load_chunk<W>(p + ln.ca, a);
+    if (ln.b) load_chunk<W>(p + ln.cb, b);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      x[i] = a[i];
+      x[W + i] = b[i];
     }
   }
 }
+template <int W, bool INTER, typename E> __device__ __forceinline__ void store_lane(E* p, const RopeLane<W, INTER>& ln, const float (&x)[2 * W]) {
+  if constexpr (INTER && W <= 4) {
+    if (ln.a) store_chunk<2 * W>(p + ln.ca, x);
+  } else {
+    float a[W], b[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a[i] = x[i];
+      b[i] = x[W + i];
+    }
+    if (ln.a) store_chunk<W>(p + ln.ca, a);
+    if (ln.b) store_chunk<W>(p + ln.cb, b);
+  }
+}
+// sum over the GL lanes of a group, every lane gets it: exchanges inside 16 lanes are modifiers of the addition
+template <int GL> __device__ __forceinline__ float group_sum(float v) {
+  auto add = [&](auto CTRL) { v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(CTRL)::value, 0xf, 0xf, true)); };
+  add(std::integral_constant<int, 0xb1>{});                           // lane ^ 1
+  add(std::integral_constant<int, 0x4e>{});                           // lane ^ 2
+  if constexpr (GL >= 8) add(std::integral_constant<int, 0x141>{});   // 7 - lane in eights: the other four
+  if constexpr (GL >= 16) add(std::integral_constant<int, 0x140>{});  // 15 - lane in sixteens: the other eight
+  if constexpr (GL >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (GL >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
 
-template <typename E, int W, int GL /* lanes per head */, bool BACK>
+template <typename E, int W, int GL /* lanes per head */, bool INTER, bool BACK>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
   __shared__ float2 table[kTpb * (kMaxHd / 2)];
   __shared__ float red[BACK ? 256 : 1];
   const int l = threadIdx.x % GL, grp = threadIdx.x / GL;
   constexpr int NG = 256 / GL;
-  const RopeLane<W> ln(p, l);
+  const RopeLane<W, INTER> ln(p, l);
   float dw[2][2 * W] = {};
   const float inv_hd = 1.0f / (float)p.hd;
   for (long c = blockIdx.x; c * kTpb < p.rows; c += gridDim.x) {
@@ -119,43 +158,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
         const size_t col = (size_t)h * p.hd;
         const E* xp = src + (size_t)(t0 + t) * ld + col;
         E* yp = dst + (size_t)(t0 + t) * ldo + col;
-        float xa[W] = {}, xb[W] = {}, x[2 * W];
-        if (ln.a) load_chunk<W>(xp + ln.ca, xa);
-        if (ln.b) load_chunk<W>(xp + ln.cb, xb);
-        float ga[W] = {}, gb[W] = {};
-        if constexpr (BACK) {
-          const E* gp = up + (size_t)(t0 + t) * ldg + col;
-          if (ln.a) load_chunk<W>(gp + ln.ca, ga);
-          if (ln.b) load_chunk<W>(gp + ln.cb, gb);
-        }
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          x[i] = xa[i];
-          x[W + i] = xb[i];
-        }
+        float x[2 * W], g[BACK ? 2 * W : 1];
+        load_lane<W, INTER>(xp, ln, x);
+        if constexpr (BACK) load_lane<W, INTER>(up + (size_t)(t0 + t) * ldg + col, ln, g);
         float r = 1.f;
         if (p.norm) {
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-          for (int o = GL / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-          const float v = fmaf(ss, inv_hd, p.eps);
+          const float v = fmaf(group_sum<GL>(ss), inv_hd, p.eps);
           r = 1.0f / sqrtf(v);
         }
         const float2* cs = table + t * (p.rot / 2) + ln.pair;
         if constexpr (!BACK) {
 #pragma unroll
           for (int i = 0; i < 2 * W; ++i) x[i] = x[i] * r * wt[i];
-          if (ln.turn) rope_turn<W, false>(cs, p.interleaved, x);
+          if (ln.turn) rope_turn<W, INTER, false>(cs, x);
         } else {
-          float g[2 * W];
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            g[i] = ga[i];
-            g[W + i] = gb[i];
-          }
-          if (ln.turn) rope_turn<W, true>(cs, p.interleaved, g);
+          if (ln.turn) rope_turn<W, INTER, true>(cs, g);
           if (p.norm) {
             float dot = 0.f;
 #pragma unroll
@@ -165,9 +185,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
               g[i] *= wt[i];
               dot = fmaf(g[i], x[i], dot);
             }
-#pragma unroll
-            for (int o = GL / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-            dot *= inv_hd;
+            dot = group_sum<GL>(dot) * inv_hd;
 #pragma unroll
             for (int i = 0; i < 2 * W; ++i) x[i] = r * fmaf(-x[i], dot, g[i]);
           } else {
@@ -175,13 +193,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
             for (int i = 0; i < 2 * W; ++i) x[i] = g[i];
           }
         }
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          xa[i] = x[i];
-          xb[i] = x[W + i];
-        }
-        if (ln.a) store_chunk<W>(yp + ln.ca, xa);
-        if (ln.b) store_chunk<W>(yp + ln.cb, xb);
+        store_lane<W, INTER>(yp, ln, x);
       }
     }
   }
@@ -203,55 +215,53 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
   }
 }
 
-// dw[c] = sum over the workgroups' rows, in a fixed order: 16 columns x 16 row lanes per workgroup
+// dw[c] = sum over the workgroups' rows, in a fixed order: 4 columns x 64 row lanes per workgroup
 __global__ __launch_bounds__(256) void rope_dw_kernel(const float* ws, int parts, int hd, float* dqw, float* dkw) {
-  __shared__ float red[16][17];
-  const int c = blockIdx.x * 16 + threadIdx.x % 16, rl = threadIdx.x / 16;
+  __shared__ float red[256];
+  const int c = blockIdx.x * 4 + (threadIdx.x & 3), rl = threadIdx.x >> 2;
   float s = 0.f;
-  if (c < 2 * hd)
-    for (int r = rl; r < parts; r += 16) s += ws[(size_t)r * 2 * hd + c];
-  red[rl][threadIdx.x % 16] = s;
+  if (c < 2 * hd) {
+#pragma unroll 8
+    for (int r = rl; r < parts; r += 64) s += ws[(size_t)r * 2 * hd + c];
+  }
+  red[threadIdx.x] = s;
   __syncthreads();
   if (rl != 0 || c >= 2 * hd) return;
-  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+  for (int i = 1; i < 64; ++i) s += red[4 * i + threadIdx.x];
   float* out = c < hd ? dqw : dkw;
   if (out != nullptr) out[c < hd ? c : c - hd] = s;
 }
 
-constexpr int kBackGroups = 512;  // workgroups of the backward pass (two per CU): rows of ws
+constexpr int kBackGroups = 1280;  // workgroups of the backward pass (five per CU, what its registers allow): rows of ws
 
-template <typename E, int W, int GL, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
+template <typename E, int W, int GL, bool INTER, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
   const long chunks = p.rows > kTpb ? (p.rows + kTpb - 1) / kTpb : 1;  // (no rows: one workgroup that leaves zeros for the weights)
   const long grid = BACK && p.ws != nullptr ? (chunks < kBackGroups ? chunks : kBackGroups) : (chunks < (1L << 30) ? chunks : (1L << 30));
-  qk_norm_rope_kernel<E, W, GL, BACK><<<dim3((unsigned)grid), 256, 0, st>>>(p);
+  qk_norm_rope_kernel<E, W, GL, INTER, BACK><<<dim3((unsigned)grid), 256, 0, st>>>(p);
   OSUD_HIP(hipGetLastError());
   if (BACK && p.ws != nullptr) {
-    rope_dw_kernel<<<dim3((2 * p.hd + 15) / 16), 256, 0, st>>>(p.ws, (int)grid, p.hd, p.dqw, p.dkw);
+    rope_dw_kernel<<<dim3((2 * p.hd + 3) / 4), 256, 0, st>>>(p.ws, (int)grid, p.hd, p.dqw, p.dkw);
     OSUD_HIP(hipGetLastError());
   }
   return OSUD_OK;
 }
-template <typename E, int W, bool BACK> int run_rope_lanes(const RopeP& p, hipStream_t st) {
-  const int lanes = p.rot / 2 / W + ((p.hd - p.rot) / W + 1) / 2;
-  if (lanes <= 4) return run_rope<E, W, 4, BACK>(p, st);
-  if (lanes <= 8) return run_rope<E, W, 8, BACK>(p, st);
-  if (lanes <= 16) return run_rope<E, W, 16, BACK>(p, st);
-  if constexpr (W <= 4) {
-    if (lanes <= 32) return run_rope<E, W, 32, BACK>(p, st);
-    return run_rope<E, W, 64, BACK>(p, st);
-  }
-  return OSUD_ERR_ARG;
-}
 template <typename E, bool BACK> int run_rope_width(const RopeP& p, hipStream_t st) {
-  // the widest chunk that divides the pairs, the head, the rows' strides and the pointers
-  size_t all = (size_t)(p.rot / 2) | (size_t)p.hd | p.ld_q | p.ld_qo | reinterpret_cast<size_t>(p.q) / sizeof(E) | reinterpret_cast<size_t>(p.qo) / sizeof(E);
+  // the widest chunk that divides the pairs, the head, the rows' strides and the pointers; a head of hd columns takes at most hd / 2 W + 1 lanes
+  size_t all = (size_t)p.hd | p.ld_q | p.ld_qo | reinterpret_cast<size_t>(p.q) / sizeof(E) | reinterpret_cast<size_t>(p.qo) / sizeof(E);
   if (p.kv_heads) all |= p.ld_k | p.ld_ko | reinterpret_cast<size_t>(p.k) / sizeof(E) | reinterpret_cast<size_t>(p.ko) / sizeof(E);
   if (BACK) all |= p.ld_gq | reinterpret_cast<size_t>(p.gq) / sizeof(E);
   if (BACK && p.kv_heads) all |= p.ld_gk | reinterpret_cast<size_t>(p.gk) / sizeof(E);
-  if (all % 8 == 0) return run_rope_lanes<E, 8, BACK>(p, st);
-  if (all % 4 == 0) return run_rope_lanes<E, 4, BACK>(p, st);
-  if (all % 2 == 0) return run_rope_lanes<E, 2, BACK>(p, st);
-  return run_rope_lanes<E, 1, BACK>(p, st);
+  if (p.interleaved) {  // (a lane's chunks are 2 W neighbouring columns)
+    all |= (size_t)p.rot;
+    if (all % 8 == 0) return p.hd <= 64 ? run_rope<E, 4, 8, true, BACK>(p, st) : run_rope<E, 4, 16, true, BACK>(p, st);
+    if (all % 4 == 0) return run_rope<E, 2, 32, true, BACK>(p, st);
+    return run_rope<E, 1, 64, true, BACK>(p, st);
+  }
+  all |= (size_t)(p.rot / 2);
+  if (all % 8 == 0) return p.hd <= 64 ? run_rope<E, 8, 4, false, BACK>(p, st) : run_rope<E, 8, 8, false, BACK>(p, st);
+  if (all % 4 == 0) return p.hd <= 64 ? run_rope<E, 4, 8, false, BACK>(p, st) : run_rope<E, 4, 16, false, BACK>(p, st);
+  if (all % 2 == 0) return run_rope<E, 2, 32, false, BACK>(p, st);
+  return run_rope<E, 1, 64, false, BACK>(p, st);
 }
 
 }  // namespace
