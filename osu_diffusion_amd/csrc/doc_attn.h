@@ -32,6 +32,7 @@ struct DocBf16 {
   static constexpr bool kExact = false;
   static __device__ __forceinline__ f32x16 mma(const u32x4& a, const u32x4& b, f32x16 c) { return mfma_h<false>(a, b, c); }
   static __device__ __forceinline__ u32x4 pack(const f32x16& v, int s) { return pack8_h<false>(v, 8 * s); }
+  static __device__ __forceinline__ u32x4 pack_rest(const f32x16& v, int s, const u32x4& hi) { return pack8_lo(v, 8 * s, hi); }  // what pack rounded away
   static __device__ __forceinline__ float dot(const u32x4& a, const u32x4& b) {
     float r = 0.f;
 #pragma unroll
@@ -64,6 +65,7 @@ struct DocF32 {
     for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[4 * s + i]);
     return r;
   }
+  static __device__ __forceinline__ u32x4 pack_rest(const f32x16&, int, const u32x4& hi) { return hi; }
   static __device__ __forceinline__ float dot(const u32x4& a, const u32x4& b) {
     float r = 0.f;
 #pragma unroll
@@ -211,11 +213,26 @@ __device__ __forceinline__ float doc_half_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// XCD-contiguous order of `n` units: workgroup b runs on XCD b % 8 and takes the units of one contiguous eighth, so that the tiles of one
-// (document, key head) read their keys through one L2
-__device__ __forceinline__ int doc_unit(int b, int n) {
-  const int q = n >> 3, r = n & 7, xcd = b & 7, idx = b >> 3;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+// Workgroup b's unit: parts of a split fastest, then key heads, then slots, from the last one (`down`) or the first: each document's longest
+// tiles under a causal mask come first (the last of its query tiles, the first of its key tiles), so that a launch ends on short ones.
+// Consecutive workgroups sit on consecutive XCDs, so the tiles of a key head stay on the XCDs of its remainder mod 8 and read its keys
+// through their L2s.  (One contiguous eighth of the units per XCD reads each key head through one L2, but where a document's tiles
+// straddle two eighths the later one ends on the longest tile: 2 documents of 8191 positions, 12 / 4 heads of 128 columns, causal: 605 us, in this order 440.)
+struct DocUnit {
+  int part, kvh, slot;
+};
+__device__ __forceinline__ DocUnit doc_unit(const DocAttnP& p, bool down) {
+  DocUnit u;
+  int b = blockIdx.x;
+  u.part = 0;
+  if (p.split > 1) {
+    u.part = b % p.split;
+    b /= p.split;
+  }
+  const int s = b / p.kv_heads;
+  u.kvh = b - s * p.kv_heads;
+  u.slot = down ? p.slots - 1 - s : s;
+  return u;
 }
 
 // ---- masks: key j is visible to position i if j < pre or i - left <= j <= i + right (a negative bound: none)

@@ -25,12 +25,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int frow = lane & 31, half = lane >> 5;
 
-  int u = doc_unit(blockIdx.x, gridDim.x);
-  const int sp = p.split > 1 ? u % p.split : 0;
-  if (p.split > 1) u /= p.split;
-  const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);  // (last tiles first: under a causal mask they are the longest)
+  const DocUnit u = doc_unit(p, true);
+  const int sp = u.part, kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile));
   const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
 

@@ -35,10 +35,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int frow = lane & 31, half = lane >> 5;
 
-  const int u = doc_unit(blockIdx.x, gridDim.x);
-  const int kvh = u / p.slots, slot = p.slots - 1 - (u - kvh * p.slots);
+  const DocUnit u = doc_unit(p, true);
+  const int kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile));
   const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
   const int vr = row0 + wave * 32 + frow;
@@ -95,10 +95,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   const size_t at = (size_t)head * p.rows_q + qrow, n_at = (size_t)p.heads * p.rows_q;
   const float lse = p.lse[at];
   const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key seen: every p is 0)
-  if (half == 0 && vr < vrows) {
-    p.delta[at] = delta;
-    p.delta[n_at + at] = lse2;
-  }
   float slope2 = 0.f;
   if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[head] * kLog2e;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -111,6 +107,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
+  float exact = 0.f;  // sum_j p dp
   const uint32_t kb = lds0 + TL::row_base(lane), tb = lds0 + TL::tr_base(lane);
   for (int it = 0; it < nblk; ++it) {
     const int stage = it & 1;
@@ -144,14 +141,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
         }
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = doc_ds<SHAPE>(s[r], dp[r], delta, dsc[r]);
+      for (int r = 0; r < 16; ++r) {
+        exact = fmaf(s[r], dp[r], exact);
+        s[r] = doc_ds<SHAPE>(s[r], dp[r], delta, dsc[r]);
+      }
 #pragma unroll
       for (int ss = 0; ss < 32 / T::STEP; ++ss) {
-        const u32x4 f = T::pack(s, ss);
+        const u32x4 f = T::pack(s, ss), lo = T::pack_rest(s, ss, f);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) dq[dt] = T::mma(TL::tr_read(ta, kt * 32 + T::STEP * ss, dt, lane), f, dq[dt]);
+        for (int dt = 0; dt < DT; ++dt) {
+          const u32x4 kf = TL::tr_read(ta, kt * 32 + T::STEP * ss, dt, lane);
+          dq[dt] = T::mma(kf, f, dq[dt]);
+          if constexpr (!T::kExact) dq[dt] = T::mma(kf, lo, dq[dt]);
+        }
       }
     }
+  }
+  exact = doc_half_sum(exact);
+  if (half == 0 && vr < vrows) {
+    p.delta[at] = exact;
+    p.delta[n_at + at] = lse2;
   }
   __syncthreads();
   if (!alive) return;
@@ -176,12 +185,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int frow = lane & 31, half = lane >> 5;
 
-  int u = doc_unit(blockIdx.x, gridDim.x);
-  const int sp = p.split > 1 ? u % p.split : 0;
-  if (p.split > 1) u /= p.split;
-  const int kvh = u / p.slots, slot = u - kvh * p.slots;
+  const DocUnit u = doc_unit(p, false);
+  const int sp = u.part, kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.k_begin, p.n_docs, p.rows_k, 1, slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.k_begin, p.n_docs, p.rows_k, 1, u.slot, lane, tile));
   const int j0 = tile * 128;
   if (tile < 0 || j0 >= d.nk) return;
   const int jw = j0 + wave * 32;  // this wave's first key
@@ -374,9 +381,12 @@ template <typename T, int HDP, int KS, int SHAPE> int run_doc_bwd(const DocAttnP
   if (bytes_q > 64 * 1024) OSUD_BIG_LDS_ONCE(kq);
   if (bytes_k > 64 * 1024) OSUD_BIG_LDS_ONCE(kk);
   p.slots = (int)((long)p.rows_q * p.G / 128) + p.n_docs;
+  const int split = p.split;
+  p.split = 1;
   kq<<<dim3((unsigned)(p.slots * p.kv_heads)), 256, bytes_q, st>>>(p);
   OSUD_HIP(hipGetLastError());
   p.slots = p.rows_k / 128 + p.n_docs;
+  p.split = split;
   kk<<<dim3((unsigned)(p.slots * p.kv_heads * p.split)), 256, bytes_k, st>>>(p);
   OSUD_HIP(hipGetLastError());
   if (p.split > 1) {
