@@ -10,13 +10,17 @@
 // reduced to a fraction of a turn there: at 10^6 positions a product in 32 bits is off by 0.06 radians.
 #include <type_traits>
 
-#include "common.h"
+#include "attn_frag.h"
 #include "kernels.h"
 
 namespace osud {
 namespace {
 
-constexpr int kTpb = 8, kMaxHd = 128;
+constexpr int kMaxHd = 128;
+// rows per workgroup and turn, head-rows in flight per group of lanes, workgroups per CU of the backward pass (what its registers allow)
+template <bool BACK> constexpr int kTpb = BACK ? 4 : 8;
+template <bool BACK> constexpr int kFlight = BACK ? 1 : 2;
+template <int W> constexpr int kBackPerCu = W == 8 ? 4 : 5;
 
 template <int W, typename E> __device__ __forceinline__ void load_chunk(const E* p, float (&v)[W]) {
   if constexpr (W == 8) load8(p, v);
@@ -118,18 +122,55 @@ template <int GL> __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// one head in registers: x becomes the result (BACK: the gradient, from the upstream gradient g; dw gains this head's share)
+template <int W, int GL, bool INTER, bool BACK>
+__device__ __forceinline__ void head(const RopeP& p, const RopeLane<W, INTER>& ln, const float2* cs, float inv_hd, const float (&wt)[2 * W], float (&x)[2 * W],
+                                     float (&g)[BACK ? 2 * W : 1], float (&dw)[2 * W]) {
+  float r = 1.f;
+  if (p.norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
+    r = 1.0f / sqrtf(fmaf(group_sum<GL>(ss), inv_hd, p.eps));
+  }
+  if constexpr (!BACK) {
+#pragma unroll
+    for (int i = 0; i < 2 * W; ++i) x[i] = x[i] * r * wt[i];
+    if (ln.turn) rope_turn<W, INTER, false>(cs, x);
+  } else {
+    if (ln.turn) rope_turn<W, INTER, true>(cs, g);
+    if (p.norm) {
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
+        x[i] *= r;
+        dw[i] = fmaf(g[i], x[i], dw[i]);
+        g[i] *= wt[i];
+        dot = fmaf(g[i], x[i], dot);
+      }
+      dot = group_sum<GL>(dot) * inv_hd;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) x[i] = r * fmaf(-x[i], dot, g[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) x[i] = g[i];
+    }
+  }
+}
+
 template <typename E, int W, int GL /* lanes per head */, bool INTER, bool BACK>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
-  __shared__ float2 table[kTpb * (kMaxHd / 2)];
-  __shared__ float red[BACK ? 256 : 1];
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BACK ? kBackPerCu<W> : 4))) void qk_norm_rope_kernel(RopeP p) {
+  constexpr int TPB = kTpb<BACK>, FL = kFlight<BACK>;
+  __shared__ float2 table[TPB * (kMaxHd / 2)];
+  __shared__ float red[BACK ? 256 * 2 * W : 1];
   const int l = threadIdx.x % GL, grp = threadIdx.x / GL;
   constexpr int NG = 256 / GL;
   const RopeLane<W, INTER> ln(p, l);
   float dw[2][2 * W] = {};
   const float inv_hd = 1.0f / (float)p.hd;
-  for (long c = blockIdx.x; c * kTpb < p.rows; c += gridDim.x) {
-    const long t0 = c * kTpb;
-    const int n = p.rows - t0 < kTpb ? (int)(p.rows - t0) : kTpb;
+  for (long c = blockIdx.x; c * TPB < p.rows; c += gridDim.x) {
+    const long t0 = c * TPB;
+    const int n = p.rows - t0 < TPB ? (int)(p.rows - t0) : TPB;
     __syncthreads();
     rope_angles(p, t0, n, table);
     __syncthreads();
@@ -148,70 +189,51 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeP p) {
         wt[i] = w != nullptr && ln.a ? w[ln.ca + i] : 1.f;
         wt[W + i] = w != nullptr && ln.b ? w[ln.cb + i] : 1.f;
       }
-      const int st = NG / heads, sh = NG - st * heads;
-      int t = grp / heads, h = grp - t * heads;
-      for (; t < n; t += st, h += sh) {
-        if (h >= heads) {
-          h -= heads;
-          if (++t >= n) break;
-        }
-        const size_t col = (size_t)h * p.hd;
-        const E* xp = src + (size_t)(t0 + t) * ld + col;
-        E* yp = dst + (size_t)(t0 + t) * ldo + col;
-        float x[2 * W], g[BACK ? 2 * W : 1];
-        load_lane<W, INTER>(xp, ln, x);
-        if constexpr (BACK) load_lane<W, INTER>(up + (size_t)(t0 + t) * ldg + col, ln, g);
-        float r = 1.f;
-        if (p.norm) {
-          float ss = 0.f;
+      // head-rows grp, grp + NG, ... of the n * heads: FL at a time, all loaded before the first is computed
+      for (int i0 = grp; i0 < n * heads; i0 += FL * NG) {
+        float x[FL][2 * W], g[FL][BACK ? 2 * W : 1];
+        int t[FL];
+        size_t out[FL];
+        bool live[FL];
 #pragma unroll
-          for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
-          const float v = fmaf(group_sum<GL>(ss), inv_hd, p.eps);
-          r = 1.0f / sqrtf(v);
-        }
-        const float2* cs = table + t * (p.rot / 2) + ln.pair;
-        if constexpr (!BACK) {
-#pragma unroll
-          for (int i = 0; i < 2 * W; ++i) x[i] = x[i] * r * wt[i];
-          if (ln.turn) rope_turn<W, INTER, false>(cs, x);
-        } else {
-          if (ln.turn) rope_turn<W, INTER, true>(cs, g);
-          if (p.norm) {
-            float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) {
-              x[i] *= r;
-              dw[part][i] = fmaf(g[i], x[i], dw[part][i]);
-              g[i] *= wt[i];
-              dot = fmaf(g[i], x[i], dot);
-            }
-            dot = group_sum<GL>(dot) * inv_hd;
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) x[i] = r * fmaf(-x[i], dot, g[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) x[i] = g[i];
+        for (int j = 0; j < FL; ++j) {
+          const int i = i0 + j * NG;
+          live[j] = i < n * heads;
+          t[j] = live[j] ? (int)((unsigned)i / (unsigned)heads) : 0;
+          const size_t row = (size_t)(t0 + t[j]), col = live[j] ? (size_t)(i - t[j] * heads) * p.hd : 0;
+          out[j] = row * ldo + col;
+          if (live[j]) load_lane<W, INTER>(src + row * ld + col, ln, x[j]);
+          if constexpr (BACK) {
+            if (live[j]) load_lane<W, INTER>(up + row * ldg + col, ln, g[j]);
           }
         }
-        store_lane<W, INTER>(yp, ln, x);
+#pragma unroll
+        for (int j = 0; j < FL; ++j) {
+          if (!live[j]) continue;  // (a group of lanes is alive or not as one)
+          head<W, GL, INTER, BACK>(p, ln, table + t[j] * (p.rot / 2) + ln.pair, inv_hd, wt, x[j], g[j], dw[part]);
+          store_lane<W, INTER>(dst + out[j], ln, x[j]);
+        }
       }
     }
   }
   if constexpr (BACK) {  // this workgroup's sums of the weight gradients, groups added in order: one row of ws
     if (p.ws == nullptr) return;
 #pragma unroll
-    for (int part = 0; part < 2; ++part)
+    for (int part = 0; part < 2; ++part) {
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 2 * W; ++i) {
-        __syncthreads();
-        red[threadIdx.x] = dw[part][i];
-        __syncthreads();
-        if (grp == 0 && (i < W ? ln.a : ln.b)) {
-          float s = 0.f;
-          for (int g = 0; g < NG; ++g) s += red[g * GL + l];
-          p.ws[((size_t)blockIdx.x * 2 + part) * p.hd + (i < W ? ln.ca + i : ln.cb + i - W)] = s;
-        }
+      for (int i = 0; i < 2 * W; ++i) red[i * 256 + threadIdx.x] = dw[part][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < 2 * W * GL; c += 256) {  // (value i of lane q of every group)
+        const int i = c / GL, q = c - i * GL;
+        const RopeLane<W, INTER> of(p, q);
+        if (!(i < W ? of.a : of.b)) continue;
+        float s = 0.f;
+#pragma unroll 8
+        for (int g = 0; g < NG; ++g) s += red[i * 256 + g * GL + q];
+        p.ws[((size_t)blockIdx.x * 2 + part) * p.hd + (i < W ? of.ca + i : of.cb + i - W)] = s;
       }
+    }
   }
 }
 
@@ -232,11 +254,17 @@ __global__ __launch_bounds__(256) void rope_dw_kernel(const float* ws, int parts
   if (out != nullptr) out[c < hd ? c : c - hd] = s;
 }
 
-constexpr int kBackGroups = 1280;  // workgroups of the backward pass (five per CU, what its registers allow): rows of ws
+constexpr int kBackGroups = 5 * 256;  // at most so many workgroups in the backward pass: rows of ws
 
 template <typename E, int W, int GL, bool INTER, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
-  const long chunks = p.rows > kTpb ? (p.rows + kTpb - 1) / kTpb : 1;  // (no rows: one workgroup that leaves zeros for the weights)
-  const long grid = BACK && p.ws != nullptr ? (chunks < kBackGroups ? chunks : kBackGroups) : (chunks < (1L << 30) ? chunks : (1L << 30));
+  constexpr int TPB = kTpb<BACK>;
+  const long chunks = p.rows > TPB ? (p.rows + TPB - 1) / TPB : 1;  // (no rows: one workgroup that leaves zeros for the weights)
+  long most = 1L << 30;
+  if (BACK) {
+    most = (long)kBackPerCu<W> * device_cus();
+    if (most > kBackGroups) most = kBackGroups;
+  }
+  const long grid = chunks < most ? chunks : most;
   qk_norm_rope_kernel<E, W, GL, INTER, BACK><<<dim3((unsigned)grid), 256, 0, st>>>(p);
   OSUD_HIP(hipGetLastError());
   if (BACK && p.ws != nullptr) {

@@ -29,11 +29,15 @@ def _heads(name, t, like=None):
     rows, heads, hd = t.shape
     if like is not None:
         assert t.dtype == like.dtype and t.device == like.device, f"{name} must have the type and device of the queries, got {t.dtype} on {t.device}"
-    if t.numel() == 0:
-        return rows, heads, hd, heads * hd
-    assert (hd == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == hd), \
-        f"{name}: the columns of a head and the heads of a row must lie next to each other, got strides {t.stride()}"
-    return rows, heads, hd, (t.stride(0) if rows > 1 else heads * hd)
+    ld, step, one = t.stride()
+    if ld != heads * hd or step != hd or one != 1:
+        if t.numel() == 0:
+            return rows, heads, hd, heads * hd
+        assert (hd == 1 or one == 1) and (heads == 1 or step == hd), \
+            f"{name}: the columns of a head and the heads of a row must lie next to each other, got strides {t.stride()}"
+        if rows == 1:
+            ld = heads * hd
+    return rows, heads, hd, ld
 
 
 def _precision(q):
@@ -43,30 +47,44 @@ def _precision(q):
     return _TYPES[q.dtype]
 
 
+def _new(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _vector(name, t, n, dtype, device):
-    assert t.shape == (n,) and t.dtype == dtype and t.device == device and t.is_contiguous(), \
+    assert t.dim() == 1 and t.numel() == n and t.dtype == dtype and t.device == device and t.is_contiguous(), \
         f"{name} must be a contiguous ({n},) {dtype} tensor on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}"
     return t.data_ptr()
 
 
 def _call(device, fn, *args):
     """fn(*args, current stream of `device`), with `device` current."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    at = device.index
+    if torch._C._cuda_getDevice() == at:  # (what torch.cuda.current_device and current_stream ask, without their objects: a call costs as much as a launch)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc:
+        _lib.check(rc)
 
 
 def _wants_grad(*tensors):
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)):
+    if not torch.is_grad_enabled():
         return False
-    if torch.cuda.is_current_stream_capturing() and any(t is not None and t.requires_grad and t.is_leaf for t in tensors):
+    wants = leaf = False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            wants, leaf = True, leaf or t.is_leaf
+    if leaf and torch.cuda.is_current_stream_capturing():
         # a leaf's gradient is accumulated on the stream of its first use, whatever eager graph made that: inside a capture the engine's wait
         # for that stream ends the process
         raise _lib.NativeError("a captured graph cannot differentiate with respect to leaf tensors here: call the *_bwd functions inside the capture")
-    return True
+    return wants
 
 
 # ------------------------------------------------------------------ norms and rotary positions of queries and keys
@@ -117,16 +135,19 @@ def _rope(q, k, positions, freqs, q_weight, k_weight, norm, eps, interleaved, ga
     return r
 
 
-def _rope_forward(q, k, r, out):
+def _rope_results(q, k, r, out):
     if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    else:
-        q_out, k_out = out
-        assert q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "out must have the shapes of q and k"
-    r.ld_q_out = _heads("q_out", q_out, q)[3]
-    r.ld_k_out = 0 if k is None else _heads("k_out", k_out, q)[3]
-    _call(q.device, _lib.lib().osud_op_qk_norm_rope, C.byref(r), q.data_ptr(), _lib.ptr(k), q_out.data_ptr(), _lib.ptr(k_out))
+        r.ld_q_out, r.ld_k_out = r.heads * r.head_dim, r.kv_heads * r.head_dim
+        return _new(q), None if k is None else _new(k)
+    q_out, k_out = out
+    assert q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "out must have the shapes of q and k"
+    r.ld_q_out, r.ld_k_out = _heads("out[0]", q_out, q)[3], 0 if k is None else _heads("out[1]", k_out, q)[3]
+    return q_out, k_out
+
+
+def _rope_forward(q, k, r, out):
+    q_out, k_out = _rope_results(q, k, r, out)
+    _call(q.device, _lib.lib().osud_op_qk_norm_rope, C.byref(r), q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
@@ -170,14 +191,7 @@ def qk_norm_rope_bwd(d_q, d_k, q, k, positions, freqs, *, q_weight=None, k_weigh
     assert d_q.shape == q.shape and (k is None or d_k.shape == k.shape), "d_q and d_k must have the shapes of q and k"
     r.ld_dq = _heads("d_q", d_q, q)[3]
     r.ld_dk = 0 if k is None else _heads("d_k", d_k, q)[3]
-    if out is None:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    else:
-        dq, dk = out
-        assert dq.shape == q.shape and (k is None or dk.shape == k.shape), "out must have the shapes of q and k"
-    r.ld_q_out = _heads("dq", dq, q)[3]
-    r.ld_k_out = 0 if k is None else _heads("dk", dk, q)[3]
+    dq, dk = _rope_results(q, k, r, out)
     hd = q.shape[2]
     dqw = None if q_weight is None else torch.empty(hd, device=q.device)
     dkw = None if k_weight is None else torch.empty(hd, device=q.device)
@@ -186,8 +200,8 @@ def qk_norm_rope_bwd(d_q, d_k, q, k, positions, freqs, *, q_weight=None, k_weigh
     if dqw is not None or dkw is not None:
         n = L.osud_op_qk_norm_rope_ws(hd)
         ws = torch.empty(n, device=q.device)
-    _call(q.device, L.osud_op_qk_norm_rope_bwd, C.byref(r), d_q.data_ptr(), _lib.ptr(d_k), q.data_ptr(), _lib.ptr(k), dq.data_ptr(), _lib.ptr(dk),
-          _lib.ptr(dqw), _lib.ptr(dkw), _lib.ptr(ws), n)
+    _call(q.device, L.osud_op_qk_norm_rope_bwd, C.byref(r), d_q.data_ptr(), _ptr(d_k), q.data_ptr(), _ptr(k), dq.data_ptr(), _ptr(dk),
+          _ptr(dqw), _ptr(dkw), _ptr(ws), n)
     return dq, dk, dqw, dkw
 
 
@@ -238,15 +252,16 @@ def _attention(q, k, v, docs, scale, cap, left, right, slopes):
 def _attention_forward(q, k, v, docs, a, out):
     fresh = out is None
     if fresh:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _new(q)
+        a.ld_out = a.heads * a.head_dim
     else:
         assert out.shape == q.shape, f"out must have the shape of q, got {tuple(out.shape)}"
-    a.ld_out = _heads("out", out, q)[3]
+        a.ld_out = _heads("out", out, q)[3]
     lse = torch.empty(q.shape[1], q.shape[0], device=q.device)
     L = _lib.lib()
     n = L.osud_op_doc_attention_ws(C.byref(a), 0)
     ws = torch.empty(n, device=q.device) if n else None
-    _call(q.device, L.osud_op_doc_attention, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), n)
+    _call(q.device, L.osud_op_doc_attention, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(ws), n)
     if docs.rows < q.shape[0]:  # (the kernel leaves rows behind the last document alone)
         lse[:, docs.rows:] = -math.inf
         if fresh:
@@ -302,10 +317,12 @@ def attention_bwd(d_out, q, k, v, out, lse, docs, *, scale=None, cap=0.0, left=N
     a.ld_out, a.ld_d_out = _heads("out", out, q)[3], _heads("d_out", d_out, q)[3]
     fresh = grads is None
     if fresh:
-        grads = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dq, dk, dv = grads
-    assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "grads must have the shapes of q, k and v"
-    a.ld_dq, a.ld_dk, a.ld_dv = _heads("dq", dq, q)[3], _heads("dk", dk, q)[3], _heads("dv", dv, q)[3]
+        dq, dk, dv = (_new(t) for t in (q, k, v))
+        a.ld_dq, a.ld_dk, a.ld_dv = a.heads * a.head_dim, a.kv_heads * a.head_dim, a.kv_heads * a.head_dim
+    else:
+        dq, dk, dv = grads
+        assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "grads must have the shapes of q, k and v"
+        a.ld_dq, a.ld_dk, a.ld_dv = _heads("dq", dq, q)[3], _heads("dk", dk, q)[3], _heads("dv", dv, q)[3]
     L = _lib.lib()
     n = L.osud_op_doc_attention_ws(C.byref(a), 1)
     ws = torch.empty(max(n, 1), device=q.device)
