@@ -357,7 +357,8 @@ int osud_op_attention_bwd(int precision, const void* qkv, const void* d_out, con
  *     pair i = columns (i, rot_dim / 2 + i), or (2 i, 2 i + 1) with interleaved != 0;  a' = gain (a cos - b sin), b' = gain (a sin + b cos).
  * Rows are ld elements apart; head h starts at column h * head_dim (so a packed projection Q | K | V is read in place).  Angles
  * are taken in 64 bits.  precision: OSUD_PREC_BF16, OSUD_PREC_F32, or OSUD_PREC_F16 (forward only).  Sums are fp32; one rounding.
- * head_dim even, <= 128; rot_dim even, 0 .. head_dim (0: norm only; positions and freqs may be NULL); kv_heads 0: queries only.  Any row stride;
+ * head_dim even, <= 128; rot_dim even, 0 .. head_dim (0: norm only; positions and freqs may be NULL); at most 16384 heads; kv_heads 0: queries
+ * only.  Row strides below 2^27 elements;
  * 16-byte aligned rows whose rot_dim / 2 and head_dim are multiples of 8 run at memory speed, others in narrower pieces.
  * Results may be written over the inputs (same pointers and strides). */
 typedef struct osud_rope {

@@ -19,7 +19,7 @@ int check_precision(const char* who, int prec, bool back) {
 int rope_params(const char* who, const osud_rope* r, bool back, const void* q, const void* k, const void* qo, const void* ko, const void* gq, const void* gk, RopeP* p) {
   OSUD_CHECK_ARG(r != nullptr, "%s: null argument", who);
   OSUD_TRY(check_precision(who, r->precision, back));
-  OSUD_CHECK_ARG(r->heads >= 1 && r->kv_heads >= 0 && r->heads <= 65536 && r->kv_heads <= 65536, "%s: heads %d, kv_heads %d", who, r->heads, r->kv_heads);
+  OSUD_CHECK_ARG(r->heads >= 1 && r->kv_heads >= 0 && r->heads <= 16384 && r->kv_heads <= 16384, "%s: heads %d, kv_heads %d", who, r->heads, r->kv_heads);
   OSUD_CHECK_ARG(r->head_dim >= 2 && r->head_dim % 2 == 0 && r->head_dim <= 128, "%s: head_dim %d is not an even number up to 128", who, r->head_dim);
   OSUD_CHECK_ARG(r->rot_dim >= 0 && r->rot_dim % 2 == 0 && r->rot_dim <= r->head_dim, "%s: rot_dim %d is not an even number up to head_dim", who, r->rot_dim);
   OSUD_CHECK_ARG(!r->norm || r->eps > 0.f, "%s: eps must be positive", who);
@@ -27,6 +27,8 @@ int rope_params(const char* who, const osud_rope* r, bool back, const void* q, c
   const int64_t wq = (int64_t)r->heads * r->head_dim, wk = (int64_t)r->kv_heads * r->head_dim;
   OSUD_CHECK_ARG(r->ld_q >= wq && r->ld_q_out >= wq && (!back || r->ld_dq >= wq), "%s: a row stride of the queries is shorter than their heads", who);
   OSUD_CHECK_ARG(r->ld_k >= wk && r->ld_k_out >= wk && (!back || r->ld_dk >= wk), "%s: a row stride of the keys is shorter than their heads", who);
+  for (int64_t ld : {r->ld_q, r->ld_k, r->ld_q_out, r->ld_k_out, back ? r->ld_dq : 0, back ? r->ld_dk : 0})
+    OSUD_CHECK_ARG(ld < (1L << 27), "%s: a row stride of %ld elements", who, (long)ld);
   if (r->rows > 0) {
     const size_t es = type_size(r->precision);
     const bool kv = r->kv_heads > 0;

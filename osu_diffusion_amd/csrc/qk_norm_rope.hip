@@ -17,10 +17,12 @@ namespace osud {
 namespace {
 
 constexpr int kMaxHd = 128;
-// rows per workgroup and turn, head-rows in flight per group of lanes, workgroups per CU of the backward pass (what its registers allow)
-template <bool BACK> constexpr int kTpb = BACK ? 4 : 8;
-template <bool BACK> constexpr int kFlight = BACK ? 1 : 2;
-template <int W> constexpr int kBackPerCu = W == 8 ? 4 : 5;
+// rows per workgroup and turn; heads in flight per group of lanes; workgroups per CU of the backward pass.  Two heads and what registers they
+// leave: 32768 rows of 16 + 16 heads of 72 columns backward (453 MB) 115 us; one head and five workgroups 121, two and three 145; fp32 one head
+// (5003 rows, 25 us against 32).
+constexpr int kTpb = 8;
+template <typename E, bool BACK> constexpr int kFlight = BACK && sizeof(E) == 4 ? 1 : 2;
+template <int W> constexpr int kBackPerCu = W == 8 ? 3 : 4;
 
 template <int W, typename E> __device__ __forceinline__ void load_chunk(const E* p, float (&v)[W]) {
   if constexpr (W == 8) load8(p, v);
@@ -78,24 +80,44 @@ template <int W, bool INTER, bool BACK> __device__ __forceinline__ void rope_tur
     x[ib] = a * t.y + b * t.x;
   }
 }
+// N neighbouring elements as they lie in memory: loaded long before they are unpacked
+template <typename E, int N> struct RawChunk {
+  static constexpr int B = N * (int)sizeof(E);
+  static constexpr bool F = std::is_same<E, float>::value;
+  typedef typename std::conditional<F, float4, uint4>::type V16;
+  typedef typename std::conditional<F, float2, uint2>::type V8;
+  typedef typename std::conditional<F, float, uint32_t>::type V4;
+  typedef typename std::conditional<B >= 16, V16, typename std::conditional<B == 8, V8, typename std::conditional<B == 4, V4, uint16_t>::type>::type>::type V;
+  V v[B >= 16 ? B / 16 : 1];
+  __device__ __forceinline__ void load(const E* p, bool there) {
+#pragma unroll
+    for (int i = 0; i < (B >= 16 ? B / 16 : 1); ++i) v[i] = there ? reinterpret_cast<const V*>(p)[i] : V{};
+  }
+  __device__ __forceinline__ void unpack(float (&x)[N]) const { load_chunk<N>(reinterpret_cast<const E*>(v), x); }
+};
 // both chunks of a head (INTER: they are one)
-template <int W, bool INTER, typename E> __device__ __forceinline__ void load_lane(const E* p, const RopeLane<W, INTER>& ln, float (&x)[2 * W]) {
-  if constexpr (INTER && W <= 4) {
-    float v[2 * W] = {};
-    if (ln.a) load_chunk<2 * W>(p + ln.ca, v);
+template <typename E, int W, bool INTER> struct RawLane {
+  static constexpr bool kOne = INTER && W <= 4;
+  RawChunk<E, kOne ? 2 * W : W> c[kOne ? 1 : 2];
+  __device__ __forceinline__ void load(const E* p, const RopeLane<W, INTER>& ln, bool there) {
+    c[0].load(p + ln.ca, there && ln.a);
+    if constexpr (!kOne) c[1].load(p + ln.cb, there && ln.b);
+  }
+  __device__ __forceinline__ void unpack(float (&x)[2 * W]) const {
+    if constexpr (kOne) {
+      c[0].unpack(x);
+    } else {
+      float a[W], b[W];
+      c[0].unpack(a);
+      c[1].unpack(b);
 #pragma unroll
-    for (int i = 0; i < 2 * W; ++i) x[i] = v[i];
-  } else {
-    float a[W] = {}, b[W] = {};
-    if (ln.a) load_chunk<W>(p + ln.ca, a);
-    if (ln.b) load_chunk<W>(p + ln.cb, b);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      x[i] = a[i];
-      x[W + i] = b[i];
+      for (int i = 0; i < W; ++i) {
+        x[i] = a[i];
+        x[W + i] = b[i];
+      }
     }
   }
-}
+};
 template <int W, bool INTER, typename E> __device__ __forceinline__ void store_lane(E* p, const RopeLane<W, INTER>& ln, const float (&x)[2 * W]) {
   if constexpr (INTER && W <= 4) {
     if (ln.a) store_chunk<2 * W>(p + ln.ca, x);
@@ -124,21 +146,21 @@ template <int GL> __device__ __forceinline__ float group_sum(float v) {
 
 // one head in registers: x becomes the result (BACK: the gradient, from the upstream gradient g; dw gains this head's share)
 template <int W, int GL, bool INTER, bool BACK>
-__device__ __forceinline__ void head(const RopeP& p, const RopeLane<W, INTER>& ln, const float2* cs, float inv_hd, const float (&wt)[2 * W], float (&x)[2 * W],
-                                     float (&g)[BACK ? 2 * W : 1], float (&dw)[2 * W]) {
+__device__ __forceinline__ void head(const RopeP& p, bool turn, const float2* cs, float inv_hd, const float (&wt)[2 * W], float (&x)[2 * W], float (&g)[2 * W],
+                                     float (&dw)[2 * W]) {
   float r = 1.f;
   if (p.norm) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * W; ++i) ss = fmaf(x[i], x[i], ss);
-    r = 1.0f / sqrtf(fmaf(group_sum<GL>(ss), inv_hd, p.eps));
+    r = __builtin_amdgcn_rsqf(fmaf(group_sum<GL>(ss), inv_hd, p.eps));  // (one unit in the last place)
   }
   if constexpr (!BACK) {
 #pragma unroll
     for (int i = 0; i < 2 * W; ++i) x[i] = x[i] * r * wt[i];
-    if (ln.turn) rope_turn<W, INTER, false>(cs, x);
+    if (turn) rope_turn<W, INTER, false>(cs, x);
   } else {
-    if (ln.turn) rope_turn<W, INTER, true>(cs, g);
+    if (turn) rope_turn<W, INTER, true>(cs, g);
     if (p.norm) {
       float dot = 0.f;
 #pragma unroll
@@ -158,62 +180,98 @@ __device__ __forceinline__ void head(const RopeP& p, const RopeLane<W, INTER>& l
   }
 }
 
+// A turn's heads of q, then of k, go by in batches of FL per group of lanes; the next batch is on its way while one is computed, and the first is
+// before the angles are taken: a cold row costs two microseconds.
 template <typename E, int W, int GL /* lanes per head */, bool INTER, bool BACK>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BACK ? kBackPerCu<W> : 4))) void qk_norm_rope_kernel(RopeP p) {
-  constexpr int TPB = kTpb<BACK>, FL = kFlight<BACK>;
+  constexpr int TPB = kTpb, FL = kFlight<E, BACK>, NG = 256 / GL;
   __shared__ float2 table[TPB * (kMaxHd / 2)];
+  __shared__ float weights[2][kMaxHd];
   __shared__ float red[BACK ? 256 * 2 * W : 1];
+  typedef RawLane<E, W, INTER> Raw;
   const int l = threadIdx.x % GL, grp = threadIdx.x / GL;
-  constexpr int NG = 256 / GL;
   const RopeLane<W, INTER> ln(p, l);
   float dw[2][2 * W] = {};
   const float inv_hd = 1.0f / (float)p.hd;
+  for (int c = threadIdx.x; c < 2 * p.hd; c += 256) {
+    const int part = c >= p.hd, i = c - part * p.hd;
+    const float* w = part ? p.kw : p.qw;
+    weights[part][i] = w != nullptr ? w[i] : 1.f;
+  }
+  const uint32_t magic[2] = {0xffffffffu / (uint32_t)p.heads + 1u, 0xffffffffu / (uint32_t)(p.kv_heads > 0 ? p.kv_heads : 1) + 1u};
+  struct Batch {
+    Raw x[FL], g[BACK ? FL : 1];
+  };
+  struct Turn {
+    long t0;        // first row
+    int n, nq, nb;  // rows; batches of q, of both
+  };
+  auto turn_of = [&](long c) {
+    Turn u;
+    u.t0 = c * TPB;
+    u.n = p.rows - u.t0 < TPB ? (p.rows > u.t0 ? (int)(p.rows - u.t0) : 0) : TPB;
+    u.nq = (u.n * p.heads + FL * NG - 1) / (FL * NG);
+    u.nb = u.nq + (u.n * p.kv_heads + FL * NG - 1) / (FL * NG);
+    return u;
+  };
+  // token and first column of head-row j of batch b; false: none  (i < 8 heads and 8 heads^2 < 2^32: the multiplication by 2^32 / heads, rounded up, divides exactly)
+  auto where = [&](auto PART, const Turn& u, int b, int j, uint32_t& t, uint32_t& col) -> bool {
+    constexpr int part = decltype(PART)::value;
+    const uint32_t heads = part ? p.kv_heads : p.heads, i = ((uint32_t)(part ? b - u.nq : b) * FL + j) * NG + grp;
+    const bool there = i < u.n * heads;
+    t = there ? (heads == 1 ? i : __umulhi(i, magic[part])) : 0;
+    col = there ? (i - t * heads) * p.hd : 0;
+    return there;
+  };
+  auto load = [&](auto PART, const Turn& u, int b, Batch& s) {
+    constexpr int part = decltype(PART)::value;
+    const size_t ld = part ? p.ld_k : p.ld_q, ldg = part ? p.ld_gk : p.ld_gq;
+    const E* const src = reinterpret_cast<const E*>(part ? p.k : p.q) + u.t0 * ld;
+    const E* const up = BACK ? reinterpret_cast<const E*>(part ? p.gk : p.gq) + u.t0 * ldg : nullptr;
+#pragma unroll
+    for (int j = 0; j < FL; ++j) {
+      uint32_t t, col;
+      const bool there = where(PART, u, b, j, t, col);
+      s.x[j].load(src + (t * (uint32_t)ld + col), ln, there);  // (row strides stay below 2^27 elements)
+      if constexpr (BACK) s.g[j].load(up + (t * (uint32_t)ldg + col), ln, there);
+    }
+  };
+  auto compute = [&](auto PART, const Turn& u, int b, const Batch& s) {
+    constexpr int part = decltype(PART)::value;
+    const size_t ldo = part ? p.ld_ko : p.ld_qo;
+    E* const dst = reinterpret_cast<E*>(part ? p.ko : p.qo) + u.t0 * ldo;
+    float wt[2 * W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      wt[i] = weights[part][ln.a ? ln.ca + i : 0];
+      wt[W + i] = weights[part][ln.b ? ln.cb + i : 0];
+    }
+#pragma unroll
+    for (int j = 0; j < FL; ++j) {
+      uint32_t t, col;
+      if (!where(PART, u, b, j, t, col)) continue;  // (a group of lanes is alive or not as one)
+      float x[2 * W], g[2 * W];
+      s.x[j].unpack(x);
+      if constexpr (BACK) s.g[j].unpack(g);
+      head<W, GL, INTER, BACK>(p, ln.turn, table + t * (p.rot / 2) + ln.pair, inv_hd, wt, x, g, dw[part]);
+      store_lane<W, INTER>(dst + (t * (uint32_t)ldo + col), ln, x);
+    }
+  };
+  constexpr std::integral_constant<int, 0> Q{};
+  constexpr std::integral_constant<int, 1> K{};
+  Batch now, next;
   for (long c = blockIdx.x; c * TPB < p.rows; c += gridDim.x) {
-    const long t0 = c * TPB;
-    const int n = p.rows - t0 < TPB ? (int)(p.rows - t0) : TPB;
+    const Turn u = turn_of(c);
+    load(Q, u, 0, now);
     __syncthreads();
-    rope_angles(p, t0, n, table);
+    rope_angles(p, u.t0, u.n, table);
     __syncthreads();
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const int heads = part ? p.kv_heads : p.heads;
-      if (heads == 0) continue;
-      const E* const src = reinterpret_cast<const E*>(part ? p.k : p.q);
-      const E* const up = reinterpret_cast<const E*>(part ? p.gk : p.gq);
-      E* const dst = reinterpret_cast<E*>(part ? p.ko : p.qo);
-      const size_t ld = part ? p.ld_k : p.ld_q, ldg = part ? p.ld_gk : p.ld_gq, ldo = part ? p.ld_ko : p.ld_qo;
-      const float* const w = part ? p.kw : p.qw;
-      float wt[2 * W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        wt[i] = w != nullptr && ln.a ? w[ln.ca + i] : 1.f;
-        wt[W + i] = w != nullptr && ln.b ? w[ln.cb + i] : 1.f;
-      }
-      // head-rows grp, grp + NG, ... of the n * heads: FL at a time, all loaded before the first is computed
-      for (int i0 = grp; i0 < n * heads; i0 += FL * NG) {
-        float x[FL][2 * W], g[FL][BACK ? 2 * W : 1];
-        int t[FL];
-        size_t out[FL];
-        bool live[FL];
-#pragma unroll
-        for (int j = 0; j < FL; ++j) {
-          const int i = i0 + j * NG;
-          live[j] = i < n * heads;
-          t[j] = live[j] ? (int)((unsigned)i / (unsigned)heads) : 0;
-          const size_t row = (size_t)(t0 + t[j]), col = live[j] ? (size_t)(i - t[j] * heads) * p.hd : 0;
-          out[j] = row * ldo + col;
-          if (live[j]) load_lane<W, INTER>(src + row * ld + col, ln, x[j]);
-          if constexpr (BACK) {
-            if (live[j]) load_lane<W, INTER>(up + row * ldg + col, ln, g[j]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < FL; ++j) {
-          if (!live[j]) continue;  // (a group of lanes is alive or not as one)
-          head<W, GL, INTER, BACK>(p, ln, table + t[j] * (p.rot / 2) + ln.pair, inv_hd, wt, x[j], g[j], dw[part]);
-          store_lane<W, INTER>(dst + out[j], ln, x[j]);
-        }
-      }
+    for (int b = 0; b < u.nb; ++b) {
+      if (b + 1 < u.nq) load(Q, u, b + 1, next);
+      else if (b + 1 < u.nb) load(K, u, b + 1, next);
+      if (b < u.nq) compute(Q, u, b, now);
+      else compute(K, u, b, now);
+      now = next;
     }
   }
   if constexpr (BACK) {  // this workgroup's sums of the weight gradients, groups added in order: one row of ws
@@ -254,10 +312,10 @@ __global__ __launch_bounds__(256) void rope_dw_kernel(const float* ws, int parts
   if (out != nullptr) out[c < hd ? c : c - hd] = s;
 }
 
-constexpr int kBackGroups = 5 * 256;  // at most so many workgroups in the backward pass: rows of ws
+constexpr int kBackGroups = 4 * 256;  // at most so many workgroups in the backward pass: rows of ws
 
 template <typename E, int W, int GL, bool INTER, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
-  constexpr int TPB = kTpb<BACK>;
+  constexpr int TPB = kTpb;
   const long chunks = p.rows > TPB ? (p.rows + TPB - 1) / TPB : 1;  // (no rows: one workgroup that leaves zeros for the weights)
   long most = 1L << 30;
   if (BACK) {
@@ -286,7 +344,9 @@ template <typename E, bool BACK> int run_rope_width(const RopeP& p, hipStream_t 
     return run_rope<E, 1, 64, true, BACK>(p, st);
   }
   all |= (size_t)(p.rot / 2);
-  if (all % 8 == 0) return p.hd <= 64 ? run_rope<E, 8, 4, false, BACK>(p, st) : run_rope<E, 8, 8, false, BACK>(p, st);
+  if constexpr (sizeof(E) == 2) {
+    if (all % 8 == 0) return p.hd <= 64 ? run_rope<E, 8, 4, false, BACK>(p, st) : run_rope<E, 8, 8, false, BACK>(p, st);
+  }
   if (all % 4 == 0) return p.hd <= 64 ? run_rope<E, 4, 8, false, BACK>(p, st) : run_rope<E, 4, 16, false, BACK>(p, st);
   if (all % 2 == 0) return run_rope<E, 2, 32, false, BACK>(p, st);
   return run_rope<E, 1, 64, false, BACK>(p, st);
