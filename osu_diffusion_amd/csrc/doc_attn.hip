@@ -15,7 +15,7 @@ namespace osud {
 namespace {
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? ((SHAPE & kShapeSlope) != 0 ? 3 : 4) : HDP == 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? (SHAPE != 0 ? 3 : 4) : HDP == 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
@@ -90,7 +90,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;
+  float m_run = (SHAPE & kShapeFixed) != 0 ? 0.f : -INFINITY, l_run = 0.f;
+  [[maybe_unused]] const bool onesided = p.right == 0 && d.pre == 0;
 
   const uint32_t kb = lds0 + TL::row_base(lane), vb = lds0 + TILE + TL::tr_base(lane);
   int stage = 0;
@@ -105,17 +106,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
     if (cls == 0) continue;
     f32x16 s[KT];
     const int key_lane = j0 + 4 * half;
-    const float dist0 = (float)(pos - key_lane);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[kt] = T::mma(TL::row_read(ka, kt * 32, ks), qf[ks], s[kt]);
+    }
+    // scores in the log2 domain: k1 * s + base (base: this block's and row's part of a distance that has one sign)
+    constexpr bool kCap = (SHAPE & kShapeCap) != 0, kSlope = (SHAPE & kShapeSlope) != 0, kFixed = (SHAPE & kShapeFixed) != 0;
+    if constexpr (kCap) {
+      float big = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float rr;
-        s[kt][r] = doc_score<T, SHAPE>(p, s[kt][r], slope2, dist0 - (float)(kt * 32 + 8 * (r >> 2) + (r & 3)), rr);
+      for (int kt = 0; kt < KT; ++kt) big = doc_largest(s[kt], big);
+      const bool small = !__any(big > p.small);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) doc_tanh<T>(p, p.tanh2, p.cap2, small, s[kt]);
+    }
+    const float k1 = kCap || kSlope ? 1.0f : p.c1;
+    float base = 0.f;
+    if constexpr (kSlope) {
+      const float dist0 = (float)(pos - key_lane);
+      if (onesided) {  // every visible key is at or before the position: -slope |pos - key| = -slope dist0 + slope off
+        base = -slope2 * dist0;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kt][r] = fmaf(s[kt][r], kCap ? 1.0f : p.c1, slope2 * (float)(kt * 32 + 8 * (r >> 2) + (r & 3)));
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[kt][r] = fmaf(-slope2, fabsf(dist0 - (float)(kt * 32 + 8 * (r >> 2) + (r & 3))), kCap ? s[kt][r] : s[kt][r] * p.c1);
       }
     }
     if (cls == 1) {
@@ -128,33 +150,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
           s[kt][r] = seen ? s[kt][r] : -INFINITY;
         }
     }
-    float mx = -INFINITY;
+    float shift = 0.f;
+    if constexpr (!kFixed) {
+      float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-    mx = doc_half_max(mx);
-    // The reference point moves only when a score passes it by 8 binary orders: p <= 2^8 stays far inside every type's range, and the
-    // accumulators are rescaled a few times per row instead of once per block
-    const bool up = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
-    if (__any(up)) {
-      const float m_new = fmaxf(m_run, mx);
-      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
-      m_run = m_new;
-      l_run *= alpha;
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+      mx = doc_half_max(fmaf(mx, k1, base));
+      // The reference point moves only when a score passes it by 8 binary orders: p <= 2^8 stays far inside every type's range, and the
+      // accumulators are rescaled a few times per row instead of once per block
+      const bool up = mx > m_run + 8.0f || (m_run == -INFINITY && mx > -INFINITY);
+      if (__any(up)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
-      for (int i = 0; i < DT; ++i)
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[i][r]) : "v"(alpha));  // (in place: as plain products the compiler copies all of o on every block)
+          for (int r = 0; r < 16; ++r) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[i][r]) : "v"(alpha));  // (in place: as plain products the compiler copies all of o on every block)
+      }
+      shift = base - (m_run == -INFINITY ? 0.f : m_run);
     }
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int ss = 0; ss < 32 / T::STEP; ++ss) {
 #pragma unroll
         for (int r = ss * T::STEP / 2; r < (ss + 1) * T::STEP / 2; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[kt][r] - m_use);
+          const float e = __builtin_amdgcn_exp2f(kFixed ? s[kt][r] : kCap || kSlope ? s[kt][r] + shift : fmaf(s[kt][r], k1, shift));
           s[kt][r] = e;
           l_run += e;
         }
@@ -236,7 +261,9 @@ template <typename T, int HDP, int KS, int SHAPE> int run_doc_attn(const DocAttn
 template <typename T, int HDP, int KS> int run_doc_attn_shape(const DocAttnP& p, hipStream_t st) {
   switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
     case 0: return run_doc_attn<T, HDP, KS, 0>(p, st);
-    case kShapeCap: return run_doc_attn<T, HDP, KS, kShapeCap>(p, st);
+    case kShapeCap:
+      if (!std::is_same<T, DocF16>::value && p.cap <= kFixedCap) return run_doc_attn<T, HDP, KS, kShapeCap | kShapeFixed>(p, st);
+      return run_doc_attn<T, HDP, KS, kShapeCap>(p, st);
     case kShapeSlope: return run_doc_attn<T, HDP, KS, kShapeSlope>(p, st);
     default: return run_doc_attn<T, HDP, KS, kShapeCap | kShapeSlope>(p, st);
   }

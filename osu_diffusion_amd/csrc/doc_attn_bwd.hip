@@ -11,13 +11,21 @@
 namespace osud {
 namespace {
 
-// p of one pair, and (cap) the factor 1 - tanh^2.  `qk`: q.k;  lse2 = lse * log2(e)
-template <typename T, int SHAPE>
-__device__ __forceinline__ float doc_weight(const DocAttnP& p, float qk, float slope2, float distance, float lse2, float& dsc) {
-  float r = 0.f;
-  const float v = doc_score<T, SHAPE>(p, qk, slope2, distance, r);
-  dsc = (SHAPE & kShapeCap) != 0 ? 4.0f * r * (1.0f - r) : 1.0f;
-  return __builtin_amdgcn_exp2f(v - lse2);
+// s[0 .. 15] (q.k) -> p = exp(score - lse); capped: dsc = 1 - tanh^2.  dist(r), lse2(r): position - key, lse * log2(e) of element r
+template <typename T, int SHAPE, typename DIST, typename LSE>
+__device__ __forceinline__ void doc_weights(const DocAttnP& p, f32x16& s, float (&dsc)[16], float slope2, DIST dist, LSE lse2) {
+  constexpr bool kCap = (SHAPE & kShapeCap) != 0, kSlope = (SHAPE & kShapeSlope) != 0;
+  if constexpr (kCap) {
+    const bool small = !__any(doc_largest(s, 0.f) > p.small);
+    doc_tanh<T>(p, p.tanh1, 1.0f, small, s);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    dsc[r] = kCap ? fmaf(-s[r], s[r], 1.0f) : 1.0f;
+    float v = fmaf(s[r], kCap ? p.cap2 : p.c1, -lse2(r));
+    if constexpr (kSlope) v = fmaf(-slope2, fabsf(dist(r)), v);
+    s[r] = __builtin_amdgcn_exp2f(v);
+  }
 }
 template <int SHAPE> __device__ __forceinline__ float doc_ds(float prob, float dp, float delta, float dsc) {
   const float ds = prob * (dp - delta);
@@ -25,7 +33,7 @@ template <int SHAPE> __device__ __forceinline__ float doc_ds(float prob, float d
 }
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 && T::ES == 4 ? 1 : 2))) void doc_attn_dq_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? 3 : 2) : (HDP == 128 ? 1 : 2)))) void doc_attn_dq_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
@@ -130,8 +138,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
       const int key_lane = j0 + kt * 32 + 4 * half;
       const float dist0 = (float)(pos - key_lane);
       float dsc[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = doc_weight<T, SHAPE>(p, s[r], slope2, dist0 - (float)(8 * (r >> 2) + (r & 3)), lse2, dsc[r]);
+      doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 - (float)(8 * (r >> 2) + (r & 3)); }, [&](int) { return lse2; });
       if (cls == 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -286,13 +293,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
       const int qi0 = i + 4 * half;
       const float dist0 = (float)(shift + qi0 - key);
       float dsc[16];
+      f32x4 ls[4];
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s[4 * q4 + e] = doc_weight<T, SHAPE>(p, s[4 * q4 + e], slope2, dist0 + (float)(8 * q4 + e), ls[e], dsc[4 * q4 + e]);
-      }
+      for (int q4 = 0; q4 < 4; ++q4) ls[q4] = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
+      doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 + (float)(8 * (r >> 2) + (r & 3)); }, [&](int r) { return ls[r >> 2][r & 3]; });
       if (cls == 1) {
         const int none = key < d.nk ? d.nq : 0;  // queries below this one exist, for a key that exists
 #pragma unroll

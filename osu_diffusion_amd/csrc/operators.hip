@@ -49,7 +49,7 @@ int doc_params(const char* who, const osud_doc_attention* a, bool back, DocAttnP
   OSUD_CHECK_ARG(a->head_dim >= 8 && a->head_dim % 8 == 0 && a->head_dim <= 128, "%s: head_dim %d is not a multiple of 8 up to 128", who, a->head_dim);
   OSUD_CHECK_ARG(a->n_docs >= 0 && a->n_docs < (1 << 24) && a->rows_q >= 0 && a->rows_k >= 0 && a->rows_q < (1 << 30) && a->rows_k < (1 << 30), "%s: %d documents, %d query and %d key rows",
                  who, a->n_docs, a->rows_q, a->rows_k);
-  OSUD_CHECK_ARG(a->scale == a->scale && a->cap == a->cap && a->cap >= 0.f, "%s: scale and cap must be numbers, cap not negative", who);
+  OSUD_CHECK_ARG(a->scale > 0.f && a->scale < 1e18f && a->cap >= 0.f && a->cap < 1e18f, "%s: scale %g must be positive, cap %g not negative", who, a->scale, a->cap);
   OSUD_CHECK_ARG(a->n_docs == 0 || (a->q_begin && a->k_begin), "%s: null offsets", who);
   const int64_t unit = 16 / (int64_t)type_size(a->precision), wq = (int64_t)a->heads * a->head_dim, wk = (int64_t)a->kv_heads * a->head_dim;
   auto stride = [&](int64_t ld, int64_t w) { return ld >= w && ld % unit == 0 && ld < (1 << 23); };
@@ -74,8 +74,18 @@ int doc_params(const char* who, const osud_doc_attention* a, bool back, DocAttnP
   z.c1 = a->scale * kLog2e;
   z.cap = a->cap;
   if (a->cap > 0.f) {
-    z.c2 = 2.0f * a->scale * kLog2e / a->cap;
+    const double x = (double)a->scale / a->cap;
+    z.c2 = (float)(2.0 * x * 1.4426950408889634);
     z.cap2 = a->cap * kLog2e;
+    z.small = (float)(0.5 / x);
+    const double four[5] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993, -0.04440222680568695, 0.0};
+    const double five[5] = {1.0, -0.3333306908607483, 0.13324779272079468, -0.05298607423901558, 0.017135007306933403};
+    double power = x;
+    for (int i = 0; i < 5; ++i, power *= x * x) {
+      const double c = (a->precision == OSUD_PREC_F32 ? five : four)[i] * power;
+      z.tanh1[i] = (float)c;
+      z.tanh2[i] = (float)(c * a->cap * 1.4426950408889634);
+    }
   }
   *p = z;
   return OSUD_OK;

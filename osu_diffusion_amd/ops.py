@@ -292,7 +292,7 @@ def attention(q, k, v, docs, *, scale=None, cap=0.0, left=None, right=None, slop
     """Attention within every document of ``docs`` (a ``Documents``): softmax over the visible keys of the scores, times v.
 
     q (rows, heads, head_dim); k, v (kv rows, kv_heads, head_dim), query head h reads key head h // (heads // kv_heads); head_dim a multiple of 8 up
-    to 128.  Query i of a document's nq stands at position nk - nq + i of its nk keys.  Scores: ``scale`` (1 / sqrt(head_dim)) times q.k; with ``cap``
+    to 128.  Query i of a document's nq stands at position nk - nq + i of its nk keys.  Scores: ``scale`` (> 0; 1 / sqrt(head_dim)) times q.k; with ``cap``
     > 0 then cap * tanh(s / cap); with ``slopes`` (heads,) float32 then minus slope * |distance|.  A key is visible within ``left`` positions before
     and ``right`` behind the query's own (None: no bound; right=0: causal), or inside the document's prefix.  A query that sees no key gets
     zeros.  Returns out (rows, heads, head_dim), zeros behind the last document (with ``out`` given those rows stay as they are); with ``return_lse``
