@@ -169,6 +169,13 @@ template <typename T, int HDP, int ROWS, int W> struct DocStage {
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(first), "s"(dst) : "memory");
     }
   }
+  // the same with the offsets worked out anew: nothing is held in registers between two calls
+  static __device__ __forceinline__ void load_fresh(const char* first, int valid, uint32_t ldb, int cols, uint32_t lds, int wave, int lane) {
+    asm volatile("" : "+v"(lane));
+    uint32_t vo[PER];
+    offsets(wave, lane, ldb, vo);
+    load(first, valid, ldb, cols, lds, wave, lane, vo);
+  }
   static __device__ __forceinline__ void clear_pads(char* tile, int cols, int tid, int threads) {
     if (cols == TL::CPR) return;
     for (int c = tid; c < ROWS * TL::CPR; c += threads) {

@@ -179,12 +179,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   });
 }
 
+// 128 columns of 16-bit elements: dk, dv and the fragments of k and v are 192 registers, one wave per SIMD.  v's fragments stay in LDS then and the
+// query blocks are halved to make room: two workgroups per CU (8192 positions, 8 / 2 heads, causal: 486 us with one wave per SIMD).
+template <typename T, int HDP> constexpr bool doc_v_in_lds = HDP == 128 && T::ES == 2;
+template <typename T, int HDP> constexpr int doc_bq = doc_v_in_lds<T, HDP> ? 32 : T::BK;
+
 // One workgroup = 128 keys of one document and key head (a wave owns 32: lane = key); the shared heads one after the other, for each the
 // query blocks that see the keys.  With a split (few key tiles), part `sp` takes its share of the (head, block) list and leaves fp32 sums.
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 || T::ES == 4 ? 1 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 ? 1 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
-  constexpr int BQ = T::BK, QT = BQ / 32, DT = HDP / 32;
+  constexpr bool VL = doc_v_in_lds<T, HDP>;
+  constexpr int BQ = doc_bq<T, HDP>, QT = BQ / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BQ, 4>;
   constexpr int TILE = ST::BYTES, STAGE = 2 * TILE + 2 * BQ * 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -217,16 +223,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 
   const int cols = p.hd * T::ES / 16;
   const uint32_t ldqb = (uint32_t)(p.ld_q * T::ES), ldgb = (uint32_t)(p.ld_do * T::ES);
-  uint32_t voq[ST::PER], vog[ST::PER];
-  ST::offsets(wave, lane, ldqb, voq);
-  ST::offsets(wave, lane, ldgb, vog);
+  uint32_t voq[VL ? 1 : ST::PER], vog[VL ? 1 : ST::PER];
+  if constexpr (!VL) {
+    ST::offsets(wave, lane, ldqb, voq);
+    ST::offsets(wave, lane, ldgb, vog);
+  }
   const size_t n_at = (size_t)p.heads * p.rows_q;
-  auto issue = [&](int i, int stage) {
-    const int g = i / nb, i0 = (b0 + i - g * nb) * BQ, head = kvh * p.G + g;
+  // (head of the group, query block) of a part's turns, one after the other
+  struct Turn {
+    int g, b;
+  };
+  auto turn_of = [&](int i) { return Turn{nb > 0 ? i / nb : 0, nb > 0 ? i % nb : 0}; };
+  auto after = [&](Turn t) { return t.b + 1 < nb ? Turn{t.g, t.b + 1} : Turn{t.g + 1, 0}; };
+  auto issue = [&](Turn t, int stage) {
+    const int i0 = (b0 + t.b) * BQ, head = kvh * p.G + t.g;
     const size_t row = (size_t)d.q0 + i0;
     const uint32_t lds = lds0 + stage * STAGE;
-    ST::load(reinterpret_cast<const char*>(p.q) + (row * p.ld_q + (size_t)head * p.hd) * T::ES, d.nq - i0, ldqb, cols, lds, wave, lane, voq);
-    ST::load(reinterpret_cast<const char*>(p.d_o) + (row * p.ld_do + (size_t)head * p.hd) * T::ES, d.nq - i0, ldgb, cols, lds + TILE, wave, lane, vog);
+    const char* const qp = reinterpret_cast<const char*>(p.q) + (row * p.ld_q + (size_t)head * p.hd) * T::ES;
+    const char* const gp = reinterpret_cast<const char*>(p.d_o) + (row * p.ld_do + (size_t)head * p.hd) * T::ES;
+    if constexpr (VL) {
+      ST::load_fresh(qp, d.nq - i0, ldqb, cols, lds, wave, lane);
+      ST::load_fresh(gp, d.nq - i0, ldgb, cols, lds + TILE, wave, lane);
+    } else {
+      ST::load(qp, d.nq - i0, ldqb, cols, lds, wave, lane, voq);
+      ST::load(gp, d.nq - i0, ldgb, cols, lds + TILE, wave, lane, vog);
+    }
     if (wave < 2 && lane < BQ) {  // wave 0: delta, wave 1: lse2 of the block's rows
       const float* src = p.delta + (wave == 1 ? n_at : 0) + (size_t)head * p.rows_q + row;
       const uint32_t off = (uint32_t)(i0 + lane < d.nq ? lane : d.nq - 1 - i0) * 4u;
@@ -237,40 +258,64 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
     ST::clear_pads(smem + i * STAGE, cols, tid, 256);
     ST::clear_pads(smem + i * STAGE + TILE, cols, tid, 256);
   }
-  if (it < it_end) issue(it, 0);
+  const uint32_t ldvb = (uint32_t)(p.ld_v * T::ES);
+  if constexpr (VL) {
+    using SV = DocStage<T, HDP, 128, 4>;
+    SV::clear_pads(smem + 2 * STAGE, cols, tid, 256);
+    SV::load_fresh(reinterpret_cast<const char*>(p.v) + (((size_t)d.k0 + j0) * p.ld_v + (size_t)kvh * p.hd) * T::ES, d.nk - j0, ldvb, cols, lds0 + 2 * STAGE, wave, lane);
+  }
+  Turn now = turn_of(it), next = now;
+  if (it < it_end) issue(now, 0);
 
-  u32x4 kf[KS], vf[KS];
+  u32x4 kf[KS], vf[VL ? 1 : KS];
   {
     const char* kp = reinterpret_cast<const char*>(p.k) + (((size_t)d.k0 + keyc) * p.ld_k + (size_t)kvh * p.hd) * T::ES;
     const char* vp = reinterpret_cast<const char*>(p.v) + (((size_t)d.k0 + keyc) * p.ld_v + (size_t)kvh * p.hd) * T::ES;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      kf[ks] = vf[ks] = u32x4{0u, 0u, 0u, 0u};
       const int c = 2 * ks + half;
-      if (c < cols) {
-        kf[ks] = *reinterpret_cast<const u32x4*>(kp + c * 16);
-        vf[ks] = *reinterpret_cast<const u32x4*>(vp + c * 16);
+      kf[ks] = u32x4{0u, 0u, 0u, 0u};
+      if (c < cols) kf[ks] = *reinterpret_cast<const u32x4*>(kp + c * 16);
+      if constexpr (!VL) {
+        vf[ks] = u32x4{0u, 0u, 0u, 0u};
+        if (c < cols) vf[ks] = *reinterpret_cast<const u32x4*>(vp + c * 16);
       }
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[ks]), "+v"(vf[ks]));
+  for (int ks = 0; ks < KS; ++ks) {
+    asm volatile("" : "+v"(kf[ks]));
+    if constexpr (!VL) asm volatile("" : "+v"(vf[ks]));
+  }
 
   f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+  if (!alive) {  // (a wave behind the last key only fetches)
+    for (int stage = 1; it < it_end; ++it, stage ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      now = after(now);
+      if (it + 1 < it_end) issue(now, stage);
+    }
+    __syncthreads();
+    return;
+  }
   const uint32_t qb = lds0 + TL::row_base(lane), tb = lds0 + TL::tr_base(lane);
+  [[maybe_unused]] const uint32_t vb = qb + 2 * STAGE + wave * 32 * TL::RB;
   // queries whose band holds this lane's key
   const int band_lo = p.right < 0 ? 0 : key - p.right - shift, band_hi = p.left < 0 ? d.nq : key + p.left - shift;
   int stage = 0;
   for (; it < it_end; ++it) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (it + 1 < it_end) issue(it + 1, stage ^ 1);
-    const int g = it / nb, i0 = (b0 + it - g * nb) * BQ;
+    next = after(now);
+    if (it + 1 < it_end) issue(next, stage ^ 1);
+    const int g = now.g, i0 = (b0 + now.b) * BQ;
+    now = next;
     float slope2 = 0.f;
     if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[kvh * p.G + g] * kLog2e;
     const uint32_t qa = qb + stage * STAGE, ga = qa + TILE, tq = tb + stage * STAGE, tg = tq + TILE;
@@ -279,17 +324,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int i = i0 + qt * 32;  // this sub-block's first query
-      if (!alive || i >= d.nq) continue;
       int cls = doc_class(p, shift + i, shift + (i + 31 < d.nq ? i + 31 : d.nq - 1), jw, jw + 31, d.nk, d.pre);
-      if (cls == 0) continue;
+      if constexpr (!VL) {  // (VL: no way round the products of a sub-block that sees nothing, the branch would cost registers)
+        if (i >= d.nq || cls == 0) continue;
+      }
       if (i + 31 >= d.nq) cls = 1;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+      if constexpr (VL) {  // one step's fragments ahead of the products and no more: 256 registers hold (left to itself the compiler fetches all and spills k)
+        u32x4 qn = TL::row_read(qa, qt * 32, 0), gn = TL::row_read(ga, qt * 32, 0), vn = TL::row_read(vb, 0, 0);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = T::mma(TL::row_read(qa, qt * 32, ks), kf[ks], s);
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 qc = qn, gc = gn, vc = vn;
+          if (ks + 1 < KS) {
+            qn = TL::row_read(qa, qt * 32, ks + 1);
+            gn = TL::row_read(ga, qt * 32, ks + 1);
+            vn = TL::row_read(vb, 0, ks + 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          s = T::mma(qc, kf[ks], s);
+          dp = T::mma(gc, vc, dp);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = T::mma(TL::row_read(ga, qt * 32, ks), vf[ks], dp);
+        for (int ks = 0; ks < KS; ++ks) s = T::mma(TL::row_read(qa, qt * 32, ks), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) dp = T::mma(TL::row_read(ga, qt * 32, ks), vf[ks], dp);
+      }
       const int qi0 = i + 4 * half;
       const float dist0 = (float)(shift + qi0 - key);
       float dsc[16];
@@ -297,7 +360,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) ls[q4] = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
       doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 + (float)(8 * (r >> 2) + (r & 3)); }, [&](int r) { return ls[r >> 2][r & 3]; });
-      if (cls == 1) {
+      if (cls != 2) {
         const int none = key < d.nk ? d.nq : 0;  // queries below this one exist, for a key that exists
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -312,18 +375,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP == 128 
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = doc_ds<SHAPE>(s[4 * q4 + e], dp[4 * q4 + e], de[e], dsc[4 * q4 + e]);
       }
+      if constexpr (VL) {
+        constexpr int N = 32 / T::STEP * DT;
+        u32x4 gn = TL::tr_read(tg, qt * 32, 0, lane), qn = TL::tr_read(tq, qt * 32, 0, lane), pf, df;
 #pragma unroll
-      for (int ss = 0; ss < 32 / T::STEP; ++ss) {
-        const u32x4 pf = T::pack(s, ss), df = T::pack(dp, ss);
+        for (int n = 0; n < N; ++n) {
+          const int ss = n / DT, dt = n % DT;
+          const u32x4 gc = gn, qc = qn;
+          if (dt == 0) {
+            pf = T::pack(s, ss);
+            df = T::pack(dp, ss);
+          }
+          if (n + 1 < N) {
+            gn = TL::tr_read(tg, qt * 32 + T::STEP * ((n + 1) / DT), (n + 1) % DT, lane);
+            qn = TL::tr_read(tq, qt * 32 + T::STEP * ((n + 1) / DT), (n + 1) % DT, lane);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          dv[dt] = T::mma(gc, pf, dv[dt]);
+          dk[dt] = T::mma(qc, df, dk[dt]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) dv[dt] = T::mma(TL::tr_read(tg, qt * 32 + T::STEP * ss, dt, lane), pf, dv[dt]);
+        for (int ss = 0; ss < 32 / T::STEP; ++ss) {
+          const u32x4 pf = T::pack(s, ss), df = T::pack(dp, ss);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) dk[dt] = T::mma(TL::tr_read(tq, qt * 32 + T::STEP * ss, dt, lane), df, dk[dt]);
+          for (int dt = 0; dt < DT; ++dt) dv[dt] = T::mma(TL::tr_read(tg, qt * 32 + T::STEP * ss, dt, lane), pf, dv[dt]);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) dk[dt] = T::mma(TL::tr_read(tq, qt * 32 + T::STEP * ss, dt, lane), df, dk[dt]);
+        }
       }
     }
   }
   __syncthreads();
-  if (!alive) return;
   if (p.split == 1) {
     char* const patch = smem + wave * 32 * TL::RB;
     auto row = [&](void* base, size_t ld) {
@@ -379,7 +463,8 @@ template <typename T, int HDP, int KS, int SHAPE> int run_doc_bwd(const DocAttnP
   using TL = DocTile<T, HDP>;
   DocAttnP p = p0;
   constexpr int tiles = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * TL::RB;
-  constexpr int bytes_q = tiles > patch ? tiles : patch, bytes_k = (tiles > patch ? tiles : patch) + 4 * T::BK * 4;
+  constexpr int BQ = doc_bq<T, HDP>, stages = 4 * DocStage<T, HDP, BQ, 4>::BYTES + 4 * BQ * 4 + (doc_v_in_lds<T, HDP> ? 128 * TL::RB : 0);
+  constexpr int bytes_q = tiles > patch ? tiles : patch, bytes_k = stages > patch ? stages : patch;
   const auto kq = doc_attn_dq_kernel<T, HDP, KS, SHAPE>;
   const auto kk = doc_attn_dkv_kernel<T, HDP, KS, SHAPE>;
   if (bytes_q > 64 * 1024) OSUD_BIG_LDS_ONCE(kq);
