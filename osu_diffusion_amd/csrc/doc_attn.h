@@ -257,6 +257,27 @@ __device__ __forceinline__ DocBand doc_band(const DocAttnP& p, int pos, int nk) 
   b.hi = p.right < 0 || pos + p.right > nk - 1 ? nk - 1 : pos + p.right;
   return b;
 }
+// the same as a start and a length, so that one comparison of unsigned numbers asks for both ends (nothing visible: a start that no key reaches)
+struct DocSpan {
+  int lo;
+  unsigned len;
+};
+__device__ __forceinline__ DocSpan doc_span(int lo, int hi) { return hi < lo ? DocSpan{1 << 30, 0u} : DocSpan{lo, (unsigned)(hi - lo)}; }
+// s[r] of the keys key0 + 8 (r / 4) + r % 4 outside of the span (and behind the prefix) becomes `none`
+__device__ __forceinline__ void doc_mask(f32x16& s, int key0, DocSpan span, int pre, float none) {
+  const int rel = key0 - span.lo;
+  if (pre > 0) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int off = 8 * (r >> 2) + (r & 3);
+      const bool seen = (key0 + off < pre) | ((unsigned)(rel + off) <= span.len);
+      s[r] = seen ? s[r] : none;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = (unsigned)(rel + 8 * (r >> 2) + (r & 3)) <= span.len ? s[r] : none;
+  }
+}
 // 0: no pair of the positions [i0, i1] and the keys [j0, j1] (cut off at nk) is visible; 2: every one is, and j1 < nk; 1: some
 __device__ __forceinline__ int doc_class(const DocAttnP& p, int i0, int i1, int j0, int j1, int nk, int pre) {
   if (j0 >= nk) return 0;

@@ -15,7 +15,7 @@ namespace osud {
 namespace {
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? (SHAPE != 0 ? 3 : 4) : HDP == 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP <= 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
@@ -85,6 +85,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));  // (waited for here, not inside the loop, where it would drain the DMA)
 
   const DocBand band = doc_band(p, pos, d.nk);
+  const DocSpan span = doc_span(band.lo, band.hi);
   f32x16 o[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i)
@@ -142,13 +143,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
     }
     if (cls == 1) {
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = key_lane + kt * 32 + 8 * (r >> 2) + (r & 3);
-          const bool seen = (key < d.pre) | ((key >= band.lo) & (key <= band.hi));
-          s[kt][r] = seen ? s[kt][r] : -INFINITY;
-        }
+      for (int kt = 0; kt < KT; ++kt) doc_mask(s[kt], key_lane + kt * 32, span, d.pre, -INFINITY);
     }
     float shift = 0.f;
     if constexpr (!kFixed) {

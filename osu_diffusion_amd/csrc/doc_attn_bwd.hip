@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]), "+v"(gf[ks]));  // (waited for here, not inside the loop, where it would drain the DMA)
 
   const DocBand band = doc_band(p, pos, d.nk);
+  const DocSpan span = doc_span(band.lo, band.hi);
   f32x16 dq[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i)
@@ -139,14 +140,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
       const float dist0 = (float)(pos - key_lane);
       float dsc[16];
       doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 - (float)(8 * (r >> 2) + (r & 3)); }, [&](int) { return lse2; });
-      if (cls == 1) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = key_lane + 8 * (r >> 2) + (r & 3);
-          const bool seen = (key < d.pre) | ((key >= band.lo) & (key <= band.hi));
-          s[r] = seen ? s[r] : 0.f;
-        }
-      }
+      if (cls == 1) doc_mask(s, key_lane, span, d.pre, 0.f);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         exact = fmaf(s[r], dp[r], exact);
@@ -306,8 +300,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 
   }
   const uint32_t qb = lds0 + TL::row_base(lane), tb = lds0 + TL::tr_base(lane);
   [[maybe_unused]] const uint32_t vb = qb + 2 * STAGE + wave * 32 * TL::RB;
-  // queries whose band holds this lane's key
-  const int band_lo = p.right < 0 ? 0 : key - p.right - shift, band_hi = p.left < 0 ? d.nq : key + p.left - shift;
+  // queries that see this lane's key
+  DocSpan span;
+  {
+    int lo = 0, hi = d.nq - 1;
+    if (key >= d.pre) {
+      if (p.right >= 0 && key - p.right - shift > lo) lo = key - p.right - shift;
+      if (p.left >= 0 && key + p.left - shift < hi) hi = key + p.left - shift;
+    }
+    span = doc_span(lo, key < d.nk ? hi : -1);
+  }
   int stage = 0;
   for (; it < it_end; ++it) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -360,15 +362,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) ls[q4] = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
       doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 + (float)(8 * (r >> 2) + (r & 3)); }, [&](int r) { return ls[r >> 2][r & 3]; });
-      if (cls != 2) {
-        const int none = key < d.nk ? d.nq : 0;  // queries below this one exist, for a key that exists
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int qi = qi0 + 8 * (r >> 2) + (r & 3);
-          const bool seen = (qi < none) & ((key < d.pre) | ((qi >= band_lo) & (qi <= band_hi)));
-          s[r] = seen ? s[r] : 0.f;
-        }
-      }
+      if (cls != 2) doc_mask(s, qi0, span, 0, 0.f);
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const f32x4 de = *reinterpret_cast<const f32x4*>(rows + qt * 32 + 8 * q4 + 4 * half);
