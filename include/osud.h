@@ -387,7 +387,7 @@ size_t osud_op_qk_norm_rope_ws(int head_dim);
  *   s = scale * q.k (scale > 0);   cap > 0: s = cap * tanh(s / cap);   slopes: s -= slopes[h] * |position - key|;
  *   key j is visible to position i if  j < prefix[d]  or  i - left <= j <= i + right   (left, right < 0: no bound; prefix NULL: 0);
  *   out = softmax over the visible keys of s, times v;   lse = log sum exp(s).
- * A row without a visible key: out 0, lse -inf, gradients 0.  Rows that belong to no document are neither read nor written.  Masked scores are
+ * A row without a visible key: out 0, lse -inf, gradients 0.  Rows behind the last document: see clear_rest.  Masked scores are
  * replaced, not added to, and documents never share a tile: what lies in another document or behind the last one has no influence, NaN included;
  * a NaN or infinity in a key or value row of the SAME document may reach every row whose 64-key block holds it.
  * Offsets out of range or out of order are clamped: results of those documents are undefined, no access leaves the tensors.
@@ -398,6 +398,7 @@ typedef struct osud_doc_attention {
   int32_t n_docs, rows_q, rows_k; /* rows of the tensors */
   int32_t left, right;
   int32_t max_q, max_k;           /* longest document, where known (0: not): only the split of the work depends on them, not the result's validity */
+  int32_t clear_rest;             /* 1: rows behind the last document get out 0, lse -inf, gradients 0; 0: they are left as they are */
   float scale, cap;
   int64_t ld_q, ld_k, ld_v, ld_out, ld_d_out, ld_dq, ld_dk, ld_dv;
   const int32_t *q_begin, *k_begin; /* (n_docs + 1) */

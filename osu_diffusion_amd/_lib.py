@@ -48,7 +48,7 @@ class Rope(C.Structure):
 
 class DocAttention(C.Structure):
     """`osud_doc_attention` of include/osud.h."""
-    _fields_ = ([(n, C.c_int32) for n in ("precision", "heads", "kv_heads", "head_dim", "n_docs", "rows_q", "rows_k", "left", "right", "max_q", "max_k")]
+    _fields_ = ([(n, C.c_int32) for n in ("precision", "heads", "kv_heads", "head_dim", "n_docs", "rows_q", "rows_k", "left", "right", "max_q", "max_k", "clear_rest")]
                 + [("scale", C.c_float), ("cap", C.c_float)]
                 + [(n, C.c_int64) for n in ("ld_q", "ld_k", "ld_v", "ld_out", "ld_d_out", "ld_dq", "ld_dk", "ld_dv")]
                 + [(n, C.c_void_p) for n in ("q_begin", "k_begin", "prefix", "slopes")])

@@ -18,7 +18,8 @@ struct DocAttnP {
   size_t ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv;  // elements between rows
   const int32_t *q_begin, *k_begin, *prefix;
   const float* slopes;
-  int rows_q, rows_k, n_docs, heads, kv_heads, G, hd, left, right, slots, split;
+  // n_docs = n_real documents, and one more where the rows behind them are to be cleared: queries without keys, keys without queries
+  int rows_q, rows_k, n_docs, n_real, heads, kv_heads, G, hd, left, right, slots, split, cus;
   float scale, c1 /* scale * log2(e) */, cap, c2 /* 2 scale log2(e) / cap */, cap2 /* cap * log2(e) */;
   float small;                // cap / 2 scale: up to this q.k the series serves
   float tanh1[5], tanh2[5];   // its coefficients for q.k -> tanh(scale q.k / cap), and that times cap2
@@ -207,13 +208,19 @@ template <int bm> __device__ __forceinline__ int doc_find(const int32_t* begin, 
   return lo;
 }
 // (offsets that are not in order or out of range give wrong results for their documents and nothing else: every row stays inside the tensors)
-__device__ __forceinline__ DocRange doc_range(const DocAttnP& p, int d) {
+__device__ __forceinline__ DocRange doc_range(const DocAttnP& p, int d, bool query_side) {
   DocRange r;
   r.q0 = doc_clamp(p.q_begin[d], 0, p.rows_q);
-  r.nq = doc_clamp(p.q_begin[d + 1], r.q0, p.rows_q) - r.q0;
   r.k0 = doc_clamp(p.k_begin[d], 0, p.rows_k);
+  r.pre = 0;
+  if (d == p.n_real) {  // the rows behind the last document
+    r.nq = query_side ? p.rows_q - r.q0 : 0;
+    r.nk = query_side ? 0 : p.rows_k - r.k0;
+    return r;
+  }
+  r.nq = doc_clamp(p.q_begin[d + 1], r.q0, p.rows_q) - r.q0;
   r.nk = doc_clamp(p.k_begin[d + 1], r.k0, p.rows_k) - r.k0;
-  r.pre = p.prefix != nullptr ? doc_clamp(p.prefix[d], 0, r.nk) : 0;
+  if (p.prefix != nullptr) r.pre = doc_clamp(p.prefix[d], 0, r.nk);
   return r;
 }
 // max / sum over lane and lane ^ 32 (v_permlane32_swap: the halves of two registers change places)
@@ -345,7 +352,7 @@ __device__ __forceinline__ void doc_store_rows(char* patch, const f32x16 (&acc)[
 }
 
 size_t doc_attn_ws(const DocAttnP& p, int prec, int max_k);   // floats of the forward's workspace (0: no split)
-size_t doc_attn_bwd_ws(const DocAttnP& p, int max_q);  // floats of the backward's: delta, lse2, parts of a split
+size_t doc_attn_bwd_ws(const DocAttnP& p, int prec, int max_q);  // floats of the backward's: delta, lse2, parts of a split
 int launch_doc_attn(int prec, DocAttnP& p, int max_k, size_t ws_floats, hipStream_t st);
 int launch_doc_attn_bwd(int prec, DocAttnP& p, int max_q, size_t ws_floats, hipStream_t st);
 

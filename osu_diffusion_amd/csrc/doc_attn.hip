@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   const DocUnit u = doc_unit(p, true);
   const int sp = u.part, kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile), true);
   const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
 
@@ -218,7 +218,8 @@ template <typename T> __global__ __launch_bounds__(256) void doc_join_kernel(Doc
   const size_t n = (size_t)p.rows_q * p.heads, at = (size_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (at >= n) return;
   const int row = (int)(at / p.heads), head = (int)(at - (size_t)row * p.heads);
-  if (row >= doc_clamp(p.q_begin[p.n_docs], 0, p.rows_q) || row < doc_clamp(p.q_begin[0], 0, p.rows_q)) return;  // (no document's: nothing was written)
+  const int end = p.n_docs > p.n_real ? p.rows_q : doc_clamp(p.q_begin[p.n_real], 0, p.rows_q);
+  if (row >= end || row < doc_clamp(p.q_begin[0], 0, p.rows_q)) return;  // (no document's: nothing was written)
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < p.split) ml = *reinterpret_cast<const float2*>(p.ws_ml + 2 * (lane * n + at));
   const float m = wave_max(ml.x), mu = m == -INFINITY ? 0.f : m;
@@ -273,26 +274,27 @@ template <typename T> int run_doc_attn_hd(const DocAttnP& p, hipStream_t st) {
 }
 
 // Parts of the key axis: few tiles (no more than one per CU) of long documents leave most of the chip idle; up to four workgroups per CU then, each
-// with at least 512 keys (a part leaves and re-reads 128 rows x head_dim floats: as much as 128 keys).
-int doc_split(const DocAttnP& p, int max_k) {
-  const int cus = device_cus(), tiles = p.slots * p.kv_heads;
+// with at least 512 keys (a part leaves and re-reads 128 rows x head_dim floats: as much as 128 keys).  fp32 keys take sixteen times as long: 128.
+int doc_split(const DocAttnP& p, int prec, int max_k) {
+  const int tiles = p.slots * p.kv_heads;
   const long keys = max_k > 0 ? max_k : p.rows_k / (p.n_docs > 0 ? p.n_docs : 1);
-  if (tiles <= 0 || tiles > cus) return 1;
-  long n = 4L * cus / tiles;
-  if (n > keys / 512) n = keys / 512;
+  if (tiles <= 0 || tiles > p.cus) return 1;
+  long n = 4L * p.cus / tiles;
+  const int least = prec == OSUD_PREC_F32 ? 128 : 512;
+  if (n > keys / least) n = keys / least;
   if (n > 64) n = 64;
   return n < 1 ? 1 : (int)n;
 }
 
 }  // namespace
 
-size_t doc_attn_ws(const DocAttnP& p, int, int max_k) {
-  const size_t n = doc_split(p, max_k);
+size_t doc_attn_ws(const DocAttnP& p, int prec, int max_k) {
+  const size_t n = doc_split(p, prec, max_k);
   return n > 1 ? n * p.rows_q * p.heads * (p.hd + 2) : 0;
 }
 
 int launch_doc_attn(int prec, DocAttnP& p, int max_k, size_t ws_floats, hipStream_t st) {
-  p.split = doc_split(p, max_k);
+  p.split = doc_split(p, prec, max_k);
   const size_t part = (size_t)p.rows_q * p.heads * (p.hd + 2);
   if (p.split > 1 && (size_t)p.split * part > ws_floats) p.split = ws_floats / part < 2 ? 1 : (int)(ws_floats / part);
   p.ws_ml = p.ws_o;

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   const DocUnit u = doc_unit(p, true);
   const int kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.q_begin, p.n_docs, p.rows_q, p.G, u.slot, lane, tile), true);
   const int vrows = d.nq * p.G, row0 = tile * 128;
   if (tile < 0 || row0 >= vrows) return;
   const int vr = row0 + wave * 32 + frow;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 
   const DocUnit u = doc_unit(p, false);
   const int sp = u.part, kvh = u.kvh;
   int tile;
-  const DocRange d = doc_range(p, doc_find<128>(p.k_begin, p.n_docs, p.rows_k, 1, u.slot, lane, tile));
+  const DocRange d = doc_range(p, doc_find<128>(p.k_begin, p.n_docs, p.rows_k, 1, u.slot, lane, tile), false);
   const int j0 = tile * 128;
   if (tile < 0 || j0 >= d.nk) return;
   const int jw = j0 + wave * 32;  // this wave's first key
@@ -435,7 +435,8 @@ template <typename T> __global__ __launch_bounds__(256) void doc_dkv_join_kernel
   if (at >= n) return;
   const size_t row = at / p.kv_heads;
   const int kvh = (int)(at - row * p.kv_heads);
-  if ((long)row >= doc_clamp(p.k_begin[p.n_docs], 0, p.rows_k) || (long)row < doc_clamp(p.k_begin[0], 0, p.rows_k)) return;
+  const int end = p.n_docs > p.n_real ? p.rows_k : doc_clamp(p.k_begin[p.n_real], 0, p.rows_k);
+  if ((int)row >= end || (int)row < doc_clamp(p.k_begin[0], 0, p.rows_k)) return;
   float acc[8] = {};
   for (int s = 0; s < p.split; ++s) {
     float v[8];
@@ -495,28 +496,28 @@ template <typename T> int run_doc_bwd_hd(const DocAttnP& p, hipStream_t st) {
   return run_doc_bwd_shape<T, 128, 128 / N>(p, st);
 }
 
-// Parts of the query axis of the key kernel: as in the forward pass, where its tiles do not give every CU four workgroups (one wave per SIMD
-// at 128 columns: the parts also even out a causal mask); at least 512 query rows per part, at most 16 parts.
-int doc_bwd_split(const DocAttnP& p, int max_q) {
-  const int cus = device_cus(), tiles = (p.rows_k / 128 + p.n_docs) * p.kv_heads;
+// Parts of the query axis of the key kernel: as in the forward pass, where its tiles do not give every CU four workgroups (the parts also even out
+// a causal mask); at least 512 query rows per part (fp32: 128), at most 16 parts.
+int doc_bwd_split(const DocAttnP& p, int prec, int max_q) {
+  const int tiles = (p.rows_k / 128 + p.n_docs) * p.kv_heads, least = prec == OSUD_PREC_F32 ? 128 : 512;
   const long rows = (long)(max_q > 0 ? max_q : p.rows_q / (p.n_docs > 0 ? p.n_docs : 1)) * p.G;
-  if (tiles <= 0 || tiles > 2 * cus) return 1;
-  long n = 4L * cus / tiles;
-  if (n > rows / 512) n = rows / 512;
+  if (tiles <= 0 || tiles > 2 * p.cus) return 1;
+  long n = 4L * p.cus / tiles;
+  if (n > rows / least) n = rows / least;
   if (n > 16) n = 16;
   return n < 1 ? 1 : (int)n;
 }
 
 }  // namespace
 
-size_t doc_attn_bwd_ws(const DocAttnP& p, int max_q) {
-  const size_t n = doc_bwd_split(p, max_q), rows = 2 * (size_t)p.heads * p.rows_q;
+size_t doc_attn_bwd_ws(const DocAttnP& p, int prec, int max_q) {
+  const size_t n = doc_bwd_split(p, prec, max_q), rows = 2 * (size_t)p.heads * p.rows_q;
   return (rows + 3) / 4 * 4 + (n > 1 ? n * p.rows_k * p.kv_heads * 2 * p.hd : 0);
 }
 
 int launch_doc_attn_bwd(int prec, DocAttnP& p, int max_q, size_t ws_floats, hipStream_t st) {
   const size_t rows = (2 * (size_t)p.heads * p.rows_q + 3) / 4 * 4, part = (size_t)p.rows_k * p.kv_heads * 2 * p.hd;
-  p.split = doc_bwd_split(p, max_q);
+  p.split = doc_bwd_split(p, prec, max_q);
   if (p.split > 1 && rows + p.split * part > ws_floats) p.split = ws_floats < rows + 2 * part ? 1 : (int)((ws_floats - rows) / part);
   p.ws_o = p.delta + rows;
   return prec == OSUD_PREC_BF16 ? run_doc_bwd_hd<DocBf16>(p, st) : run_doc_bwd_hd<DocF32>(p, st);

@@ -50,26 +50,28 @@ int doc_params(const char* who, const osud_doc_attention* a, bool back, DocAttnP
   OSUD_CHECK_ARG(a->n_docs >= 0 && a->n_docs < (1 << 24) && a->rows_q >= 0 && a->rows_k >= 0 && a->rows_q < (1 << 30) && a->rows_k < (1 << 30), "%s: %d documents, %d query and %d key rows",
                  who, a->n_docs, a->rows_q, a->rows_k);
   OSUD_CHECK_ARG(a->scale > 0.f && a->scale < 1e18f && a->cap >= 0.f && a->cap < 1e18f, "%s: scale %g must be positive, cap %g not negative", who, a->scale, a->cap);
-  OSUD_CHECK_ARG(a->n_docs == 0 || (a->q_begin && a->k_begin), "%s: null offsets", who);
+  OSUD_CHECK_ARG((a->n_docs == 0 && a->clear_rest == 0) || (a->q_begin && a->k_begin), "%s: null offsets", who);
   const int64_t unit = 16 / (int64_t)type_size(a->precision), wq = (int64_t)a->heads * a->head_dim, wk = (int64_t)a->kv_heads * a->head_dim;
   auto stride = [&](int64_t ld, int64_t w) { return ld >= w && ld % unit == 0 && ld < (1 << 23); };
   OSUD_CHECK_ARG(stride(a->ld_q, wq) && stride(a->ld_k, wk) && stride(a->ld_v, wk) && stride(a->ld_out, wq), "%s: a row stride is shorter than its heads or not a multiple of 16 bytes", who);
   OSUD_CHECK_ARG(!back || (stride(a->ld_d_out, wq) && stride(a->ld_dq, wq) && stride(a->ld_dk, wk) && stride(a->ld_dv, wk)),
                  "%s: a row stride is shorter than its heads or not a multiple of 16 bytes", who);
   const int G = a->heads / a->kv_heads;
-  const int64_t tiles = ((int64_t)a->rows_q * G / 128 + a->n_docs) * a->kv_heads, ktiles = ((int64_t)a->rows_k / 128 + a->n_docs) * a->kv_heads;
+  const int docs = a->n_docs + (a->clear_rest != 0);
+  const int64_t tiles = ((int64_t)a->rows_q * G / 128 + docs) * a->kv_heads, ktiles = ((int64_t)a->rows_k / 128 + docs) * a->kv_heads;
   OSUD_CHECK_ARG((int64_t)a->rows_q * G < (1L << 31) - 128, "%s: %d query rows of %d shared heads", who, a->rows_q, G);
   OSUD_CHECK_ARG(tiles < (1 << 24) && ktiles < (1 << 24), "%s: too many tiles for one launch", who);
   DocAttnP z = {};
   z.ld_q = a->ld_q; z.ld_k = a->ld_k; z.ld_v = a->ld_v; z.ld_o = a->ld_out;
   z.ld_do = a->ld_d_out; z.ld_dq = a->ld_dq; z.ld_dk = a->ld_dk; z.ld_dv = a->ld_dv;
   z.q_begin = a->q_begin; z.k_begin = a->k_begin; z.prefix = a->prefix; z.slopes = a->slopes;
-  z.rows_q = a->rows_q; z.rows_k = a->rows_k; z.n_docs = a->n_docs; z.heads = a->heads; z.kv_heads = a->kv_heads; z.G = G; z.hd = a->head_dim;
+  z.rows_q = a->rows_q; z.rows_k = a->rows_k; z.n_real = a->n_docs; z.n_docs = docs; z.heads = a->heads; z.kv_heads = a->kv_heads; z.G = G; z.hd = a->head_dim;
   const int far = 1 << 30;  // (positions are smaller: no bound, and position +- bound stays inside 32 bits)
   z.left = a->left < 0 || a->left >= far ? -1 : a->left;
   z.right = a->right < 0 || a->right >= far ? -1 : a->right;
-  z.slots = (int)((int64_t)a->rows_q * G / 128) + a->n_docs;
+  z.slots = (int)((int64_t)a->rows_q * G / 128) + docs;
   z.split = 1;
+  z.cus = device_cus();
   z.scale = a->scale;
   z.c1 = a->scale * kLog2e;
   z.cap = a->cap;
@@ -119,7 +121,7 @@ extern "C" int osud_op_qk_norm_rope_bwd(const osud_rope* r, const void* d_q_out,
 extern "C" size_t osud_op_doc_attention_ws(const osud_doc_attention* a, int backward) {
   DocAttnP p;
   if (doc_params("op_doc_attention_ws", a, backward != 0, &p) != OSUD_OK) return 0;
-  return backward ? doc_attn_bwd_ws(p, a->max_q) : doc_attn_ws(p, a->precision, a->max_k);
+  return backward ? doc_attn_bwd_ws(p, a->precision, a->max_q) : doc_attn_ws(p, a->precision, a->max_k);
 }
 
 extern "C" int osud_op_doc_attention(const osud_doc_attention* a, const void* q, const void* k, const void* v, void* out, float* lse, float* ws,

@@ -240,7 +240,7 @@ def _attention(q, k, v, docs, scale, cap, left, right, slopes):
     assert (left is None or left >= 0) and (right is None or right >= 0), "left and right must not be negative (None: no bound)"
     far = 1 << 30
     a = _lib.DocAttention(prec, heads, kv_heads, hd, docs.count, rows, krows, -1 if left is None else min(left, far), -1 if right is None else min(right, far),
-                          docs.max_len, docs.max_kv_len, 1.0 / math.sqrt(hd) if scale is None else scale, cap, ld_q, ld_k, ld_v)
+                          docs.max_len, docs.max_kv_len, 0, 1.0 / math.sqrt(hd) if scale is None else scale, cap, ld_q, ld_k, ld_v)
     a.q_begin, a.k_begin = docs.q_begin.data_ptr(), docs.k_begin.data_ptr()
     if docs.prefix is not None:
         a.prefix = docs.prefix.data_ptr()
@@ -254,6 +254,7 @@ def _attention_forward(q, k, v, docs, a, out):
     if fresh:
         out = _new(q)
         a.ld_out = a.heads * a.head_dim
+        a.clear_rest = docs.rows < q.shape[0]
     else:
         assert out.shape == q.shape, f"out must have the shape of q, got {tuple(out.shape)}"
         a.ld_out = _heads("out", out, q)[3]
@@ -262,10 +263,8 @@ def _attention_forward(q, k, v, docs, a, out):
     n = L.osud_op_doc_attention_ws(C.byref(a), 0)
     ws = torch.empty(n, device=q.device) if n else None
     _call(q.device, L.osud_op_doc_attention, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _ptr(ws), n)
-    if docs.rows < q.shape[0]:  # (the kernel leaves rows behind the last document alone)
+    if not fresh and docs.rows < q.shape[0]:
         lse[:, docs.rows:] = -math.inf
-        if fresh:
-            out[docs.rows:].zero_()
     return out, lse
 
 
@@ -319,6 +318,7 @@ def attention_bwd(d_out, q, k, v, out, lse, docs, *, scale=None, cap=0.0, left=N
     if fresh:
         dq, dk, dv = (_new(t) for t in (q, k, v))
         a.ld_dq, a.ld_dk, a.ld_dv = a.heads * a.head_dim, a.kv_heads * a.head_dim, a.kv_heads * a.head_dim
+        a.clear_rest = docs.rows < q.shape[0] or docs.kv_rows < k.shape[0]
     else:
         dq, dk, dv = grads
         assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "grads must have the shapes of q, k and v"
@@ -328,10 +328,4 @@ def attention_bwd(d_out, q, k, v, out, lse, docs, *, scale=None, cap=0.0, left=N
     ws = torch.empty(max(n, 1), device=q.device)
     _call(q.device, L.osud_op_doc_attention_bwd, C.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), d_out.data_ptr(),
           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), n)
-    if fresh:
-        if docs.rows < q.shape[0]:
-            dq[docs.rows:].zero_()
-        if docs.kv_rows < k.shape[0]:
-            dk[docs.kv_rows:].zero_()
-            dv[docs.kv_rows:].zero_()
     return dq, dk, dv

@@ -19,7 +19,7 @@ def rope(**kw):
 
 
 def docs(**kw):
-    a = _lib.DocAttention(_lib.PREC_BF16, 4, 2, 64, 3, 100, 100, -1, -1, 0, 0, 0.125, 0.0, 512, 512, 512, 256, 256, 256, 128, 128, P, P, None, None)
+    a = _lib.DocAttention(_lib.PREC_BF16, 4, 2, 64, 3, 100, 100, -1, -1, 0, 0, 0, 0.125, 0.0, 512, 512, 512, 256, 256, 256, 128, 128, P, P, None, None)
     for n, v in kw.items():
         setattr(a, n, v)
     return a
