@@ -15,7 +15,7 @@ namespace osud {
 namespace {
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP <= 96 ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 || (HDP == 96 && (KS == 5 || (SHAPE & kShapeSlope) == 0)) ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;

@@ -33,7 +33,7 @@ template <int SHAPE> __device__ __forceinline__ float doc_ds(float prob, float d
 }
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 ? 3 : 2) : (HDP == 128 ? 1 : 2)))) void doc_attn_dq_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 && (SHAPE & kShapeCap) == 0 ? 3 : 2) : (HDP == 128 ? 1 : 2)))) void doc_attn_dq_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
