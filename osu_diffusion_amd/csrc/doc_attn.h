@@ -270,19 +270,21 @@ struct DocSpan {
   unsigned len;
 };
 __device__ __forceinline__ DocSpan doc_span(int lo, int hi) { return hi < lo ? DocSpan{1 << 30, 0u} : DocSpan{lo, (unsigned)(hi - lo)}; }
-// s[r] of the keys key0 + 8 (r / 4) + r % 4 outside of the span (and behind the prefix) becomes `none`
-__device__ __forceinline__ void doc_mask(f32x16& s, int key0, DocSpan span, int pre, float none) {
+// s[r] of the keys key0 + 8 (r / 4) + r % 4 outside of the span and behind the prefix becomes `none`.  APART: documents without a prefix have a way of
+// their own.  (What it is worth is the compiler's registers: without caps one way keeps four waves per SIMD at 64 columns, 32 documents of 1024
+// positions 130 us against 142; under a cap it takes scalar registers that are not there, 8 documents of 4096 390 us against 350.)
+template <bool APART> __device__ __forceinline__ void doc_mask(f32x16& s, int key0, DocSpan span, int pre, float none) {
   const int rel = key0 - span.lo;
-  if (pre > 0) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int off = 8 * (r >> 2) + (r & 3);
-      const bool seen = (key0 + off < pre) | ((unsigned)(rel + off) <= span.len);
-      s[r] = seen ? s[r] : none;
-    }
-  } else {
+  if (APART && pre == 0) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = (unsigned)(rel + 8 * (r >> 2) + (r & 3)) <= span.len ? s[r] : none;
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int off = 8 * (r >> 2) + (r & 3);
+    const bool seen = (key0 + off < pre) | ((unsigned)(rel + off) <= span.len);
+    s[r] = seen ? s[r] : none;
   }
 }
 // 0: no pair of the positions [i0, i1] and the keys [j0, j1] (cut off at nk) is visible; 2: every one is, and j1 < nk; 1: some

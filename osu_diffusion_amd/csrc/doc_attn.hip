@@ -15,7 +15,7 @@ namespace osud {
 namespace {
 
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 || (HDP == 96 && (KS == 5 || (SHAPE & kShapeSlope) == 0)) ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 ? (HDP == 64 && SHAPE == 0 ? 4 : HDP == 64 || (HDP == 96 && (KS == 5 || (SHAPE & kShapeSlope) == 0)) ? 3 : 2) : (HDP == 64 ? 2 : 1)))) void doc_attn_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
   constexpr int BK = T::BK, KT = BK / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BK, 4>;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
     }
     if (cls == 1) {
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) doc_mask(s[kt], key_lane + kt * 32, span, d.pre, -INFINITY);
+      for (int kt = 0; kt < KT; ++kt) doc_mask<kCap>(s[kt], key_lane + kt * 32, span, d.pre, -INFINITY);
     }
     float shift = 0.f;
     if constexpr (!kFixed) {

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
       const float dist0 = (float)(pos - key_lane);
       float dsc[16];
       doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 - (float)(8 * (r >> 2) + (r & 3)); }, [&](int) { return lse2; });
-      if (cls == 1) doc_mask(s, key_lane, span, d.pre, 0.f);
+      if (cls == 1) doc_mask<(SHAPE & kShapeCap) != 0>(s, key_lane, span, d.pre, 0.f);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         exact = fmaf(s[r], dp[r], exact);
@@ -174,16 +174,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
 }
 
 // 128 columns of 16-bit elements: dk, dv and the fragments of k and v are 192 registers, one wave per SIMD.  v's fragments stay in LDS then and the
-// query blocks are halved to make room: two workgroups per CU (8192 positions, 8 / 2 heads, causal: 486 us with one wave per SIMD).
-template <typename T, int HDP> constexpr bool doc_v_in_lds = HDP == 128 && T::ES == 2;
-template <typename T, int HDP> constexpr int doc_bq = doc_v_in_lds<T, HDP> ? 32 : T::BK;
+// query blocks are halved to make room: two workgroups per CU (8192 positions, 8 / 2 heads, causal: 343 us; 486 with one wave per SIMD).  64
+// columns: three instead of two (256 ragged windows, backward 196 us instead of 209; capped and sloped scores need the registers: 1268 instead of 1232).
+template <typename T, int HDP, int SHAPE> constexpr bool doc_v_in_lds = T::ES == 2 && (HDP == 128 || (HDP == 64 && SHAPE == 0));
+template <typename T, int HDP> constexpr int doc_bq = HDP == 128 && T::ES == 2 ? 32 : T::BK;
 
 // One workgroup = 128 keys of one document and key head (a wave owns 32: lane = key); the shared heads one after the other, for each the
 // query blocks that see the keys.  With a split (few key tiles), part `sp` takes its share of the (head, block) list and leaves fp32 sums.
 template <typename T, int HDP, int KS, int SHAPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 ? 1 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 ? 1 : HDP == 64 && SHAPE == 0 ? 3 : 2))) void doc_attn_dkv_kernel(DocAttnP p) {
   using TL = DocTile<T, HDP>;
-  constexpr bool VL = doc_v_in_lds<T, HDP>;
+  constexpr bool VL = doc_v_in_lds<T, HDP, SHAPE>;
   constexpr int BQ = doc_bq<T, HDP>, QT = BQ / 32, DT = HDP / 32;
   using ST = DocStage<T, HDP, BQ, 4>;
   constexpr int TILE = ST::BYTES, STAGE = 2 * TILE + 2 * BQ * 4;
@@ -362,7 +363,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 4 
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) ls[q4] = *reinterpret_cast<const f32x4*>(rows + BQ + qt * 32 + 8 * q4 + 4 * half);
       doc_weights<T, SHAPE>(p, s, dsc, slope2, [&](int r) { return dist0 + (float)(8 * (r >> 2) + (r & 3)); }, [&](int r) { return ls[r >> 2][r & 3]; });
-      if (cls != 2) doc_mask(s, qi0, span, 0, 0.f);
+      if (cls != 2) doc_mask<true>(s, qi0, span, 0, 0.f);
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const f32x4 de = *reinterpret_cast<const f32x4*>(rows + qt * 32 + 8 * q4 + 4 * half);
@@ -458,7 +459,7 @@ template <typename T, int HDP, int KS, int SHAPE> int run_doc_bwd(const DocAttnP
   using TL = DocTile<T, HDP>;
   DocAttnP p = p0;
   constexpr int tiles = 4 * DocStage<T, HDP, T::BK, 4>::BYTES, patch = 4 * 32 * TL::RB;
-  constexpr int BQ = doc_bq<T, HDP>, stages = 4 * DocStage<T, HDP, BQ, 4>::BYTES + 4 * BQ * 4 + (doc_v_in_lds<T, HDP> ? 128 * TL::RB : 0);
+  constexpr int BQ = doc_bq<T, HDP>, stages = 4 * DocStage<T, HDP, BQ, 4>::BYTES + 4 * BQ * 4 + (doc_v_in_lds<T, HDP, SHAPE> ? 128 * TL::RB : 0);
   constexpr int bytes_q = tiles > patch ? tiles : patch, bytes_k = stages > patch ? stages : patch;
   const auto kq = doc_attn_dq_kernel<T, HDP, KS, SHAPE>;
   const auto kk = doc_attn_dkv_kernel<T, HDP, KS, SHAPE>;
