@@ -384,7 +384,7 @@ size_t osud_op_qk_norm_rope_ws(int head_dim);
  * A batch is n_docs documents one after the other: document d has the query rows q_begin[d] .. q_begin[d + 1] - 1 and the key / value rows
  * k_begin[d] .. k_begin[d + 1] - 1 (DEVICE arrays, int32, not decreasing; queries and keys of one document may differ in number: query i of
  * nq stands at position nk - nq + i of its nk keys).  No pair of different documents is formed.  Query head h reads key head h / (heads / kv_heads).
- *   s = scale * q.k (scale > 0);   cap > 0: s = cap * tanh(s / cap);   slopes: s -= slopes[h] * |position - key|;
+ *   s = scale * q.k (scale > 0);   cap > 0 (at least scale / 10^4): s = cap * tanh(s / cap);   slopes: s -= slopes[h] * |position - key|;
  *   key j is visible to position i if  j < prefix[d]  or  i - left <= j <= i + right   (left, right < 0: no bound; prefix NULL: 0);
  *   out = softmax over the visible keys of s, times v;   lse = log sum exp(s).
  * A row without a visible key: out 0, lse -inf, gradients 0.  Rows behind the last document: see clear_rest.  Masked scores are

@@ -47,6 +47,7 @@ int doc_params(const char* who, const osud_doc_attention* a, bool back, DocAttnP
   OSUD_TRY(check_precision(who, a->precision, back));
   OSUD_CHECK_ARG(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0 && a->heads <= 65536, "%s: heads %d is not a multiple of kv_heads %d", who, a->heads, a->kv_heads);
   OSUD_CHECK_ARG(a->head_dim >= 8 && a->head_dim % 8 == 0 && a->head_dim <= 128, "%s: head_dim %d is not a multiple of 8 up to 128", who, a->head_dim);
+  OSUD_CHECK_ARG(a->cap == 0.f || a->cap * 1e4f >= a->scale, "%s: cap %g is below scale %g / 10^4", who, a->cap, a->scale);
   OSUD_CHECK_ARG(a->n_docs >= 0 && a->n_docs < (1 << 24) && a->rows_q >= 0 && a->rows_k >= 0 && a->rows_q < (1 << 30) && a->rows_k < (1 << 30), "%s: %d documents, %d query and %d key rows",
                  who, a->n_docs, a->rows_q, a->rows_k);
   OSUD_CHECK_ARG(a->scale > 0.f && a->scale < 1e18f && a->cap >= 0.f && a->cap < 1e18f, "%s: scale %g must be positive, cap %g not negative", who, a->scale, a->cap);

@@ -122,6 +122,7 @@ def _rope(q, k, positions, freqs, q_weight, k_weight, norm, eps, interleaved, ga
         krows, r.kv_heads, khd, r.ld_k = _heads("k", k, q)
         assert (krows, khd) == (rows, hd), f"k must have the rows and the head_dim of q, got {tuple(k.shape)} and {tuple(q.shape)}"
     if freqs is not None:
+        assert not (torch.is_grad_enabled() and (freqs.requires_grad or (positions is not None and positions.requires_grad))), "positions and freqs have no gradient"
         r.rot_dim = 2 * freqs.numel()
         r.freqs = _vector("freqs", freqs, freqs.numel(), torch.float64, q.device)
         assert positions is not None and positions.dtype in (torch.int32, torch.float32), "positions must be an int32 or float32 tensor"
@@ -245,6 +246,7 @@ def _attention(q, k, v, docs, scale, cap, left, right, slopes):
     if docs.prefix is not None:
         a.prefix = docs.prefix.data_ptr()
     if slopes is not None:
+        assert not (slopes.requires_grad and torch.is_grad_enabled()), "slopes have no gradient"
         a.slopes = _vector("slopes", slopes, heads, torch.float32, q.device)
     return a
 

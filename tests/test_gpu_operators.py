@@ -110,7 +110,8 @@ def test_rope_many_rows_and_large_values():
 MASKS = {
     "all": {}, "causal": dict(right=0), "band": dict(left=20, right=7), "self": dict(left=0, right=0), "left": dict(left=33),
     "prefix": dict(right=0, prefix=True), "prefix_band": dict(left=5, right=3, prefix=True), "cap": dict(cap=5.0), "slopes": dict(slopes=True),
-    "cap_slopes_causal": dict(cap=30.0, slopes=True, right=0),
+    "cap_slopes_causal": dict(cap=30.0, slopes=True, right=0), "cap_large": dict(cap=80.0), "cap_band": dict(cap=2.0, left=10, right=4),
+    "slopes_causal": dict(slopes=True, right=0), "slopes_prefix_causal": dict(slopes=True, right=0, prefix=True),
 }
 LENGTHS = [1, 0, 31, 130, 2, 64, 0, 257, 65]
 
@@ -227,6 +228,38 @@ def test_rows_behind_the_last_document_stay_as_they_are():
         assert torch.equal(got[:103], want[:103])
 
 
+def test_documents_without_rows():
+    """No documents at all, only empty ones, queries without any key row: zeros, no gradients."""
+    q, k, v = normal(1, 10, 2, 64), normal(2, 6, 1, 64), normal(3, 6, 1, 64)
+    for lengths, kv in (([], []), ([0, 0], [0, 0]), ([4, 0], [0, 6])):
+        docs = ops.Documents(lengths, device=DEV, kv_lengths=kv)
+        out, lse = ops.attention(q, k, v, docs, return_lse=True)
+        grads = ops.attention_bwd(q, q, k, v, out, lse, docs)
+        assert not bool(out.any()) and bool((lse == -math.inf).all()) and not any(bool(g.any()) for g in grads)
+    none = torch.empty(0, 1, 64, device=DEV, dtype=BF)
+    docs = ops.Documents([10], device=DEV, kv_lengths=[0])
+    out, lse = ops.attention(q, none, none, docs, return_lse=True)
+    dq, dk, dv = ops.attention_bwd(q, q, none, none, out, lse, docs)
+    assert not bool(out.any()) and not bool(dq.any()) and dk.shape == none.shape
+    docs = ops.Documents([0], device=DEV, kv_lengths=[6])
+    out, lse = ops.attention(none, k, v, docs, return_lse=True)
+    dq, dk, dv = ops.attention_bwd(none, none, k, v, out, lse, docs)
+    assert out.shape == none.shape and not bool(dk.any()) and not bool(dv.any())
+
+
+def test_large_scores_and_every_magnitude_of_a_cap():
+    """Scores of thousands without a cap; caps from a thousandth of the scores to a thousand times them (both forms of the tanh in one tile)."""
+    lengths = [150, 70]
+    q, k, v = (t.contiguous() for t in attention_inputs(F32, 2, 2, 64, lengths, tail=0, seed=5))
+    d_out = normal(6, *q.shape, dtype=F32)
+    compare(q * 300, k, v, lengths, d_out=d_out)
+    for cap in (0.01, 1.0, 7.0, 59.0, 61.0, 1e4):
+        compare(q * 3, k, v, lengths, d_out=d_out, cap=cap)
+    q[::7] *= 30  # outliers
+    for dtype in (BF, F32):
+        compare(q.to(dtype), k.to(dtype), v.to(dtype), lengths, d_out=d_out.to(dtype), cap=20.0, right=0)
+
+
 def test_same_bits_every_time_and_on_another_stream():
     lengths = [300, 5, 1000]
     q, k, v = attention_inputs(BF, 4, 1, 128, lengths, tail=0)
@@ -303,7 +336,11 @@ def test_refusals_on_the_gpu():
     with pytest.raises(AssertionError):
         ops.attention(q, k, v, docs, slopes=torch.zeros(2, device=DEV))
     with pytest.raises(AssertionError):
+        ops.attention(q, k, v, docs, slopes=torch.zeros(4, device=DEV, requires_grad=True))
+    with pytest.raises(AssertionError):
         ops.attention(normal(1, 10, 3, 64), k, v, docs)
+    with pytest.raises(AssertionError):
+        ops.attention(normal(1, 1, 4, 64).expand(10, 4, 64), k, v, docs)  # every row the same memory
     odd = torch.zeros(10 * 4 * 64 + 1, device=DEV, dtype=BF)[1:].view(10, 4, 64)  # not 16-byte aligned
     with pytest.raises(AssertionError):
         ops.attention(odd, k, v, docs)

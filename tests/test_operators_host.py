@@ -59,7 +59,7 @@ def test_nothing_to_do_is_no_error():
 
 
 @pytest.mark.parametrize("change", [dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(head_dim=60), dict(head_dim=136), dict(head_dim=0), dict(n_docs=-1),
-                                    dict(rows_q=-1), dict(rows_k=1 << 30), dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(scale=math.nan), dict(scale=0.0), dict(scale=-1.0), dict(q_begin=None),
+                                    dict(rows_q=-1), dict(rows_k=1 << 30), dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(cap=1e-6), dict(scale=math.nan), dict(scale=0.0), dict(scale=-1.0), dict(q_begin=None),
                                     dict(k_begin=None), dict(ld_q=248), dict(ld_q=516), dict(ld_k=120), dict(ld_v=1 << 24), dict(ld_out=255)])
 def test_attention_refuses(change):
     L = _lib.lib()
