@@ -25,7 +25,11 @@ struct DocAttnP {
   float tanh1[5], tanh2[5];   // its coefficients for q.k -> tanh(scale q.k / cap), and that times cap2
 };
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+// logarithms of sums between the two bases, once per row: in 64 bits, one rounding (a relative error of 2^-24 of a logarithm of 10 is one of 6e-7 in
+// every weight of the row)
+__device__ __forceinline__ float doc_lse(float m, float l) { return l == 0.f ? -INFINITY : (float)(((double)m + (double)__builtin_amdgcn_logf(l)) * 0.6931471805599453094); }
+__device__ __forceinline__ float doc_lse2(float lse) { return lse == -INFINITY ? INFINITY : (float)((double)lse * 1.4426950408889634074); }  // (no key seen: every p is 0)
 // kShapeFixed (forward, bf16 and fp32, capped, no slopes, cap <= 60): scores lie within +- 87 binary orders, so 2^score, its sum over 2^30 keys and
 // its products with v stay inside the types' ranges without a running maximum
 enum { kShapeCap = 1, kShapeSlope = 2, kShapeFixed = 4 };

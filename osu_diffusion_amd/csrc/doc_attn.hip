@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   if (p.split == 1) {
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // (no key seen: zeros)
     if (p.lse != nullptr && half == 0 && vr < vrows)
-      p.lse[(size_t)head * p.rows_q + qrow] = l == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(l)) * kLn2;
+      p.lse[(size_t)head * p.rows_q + qrow] = doc_lse(m_run, l);
     doc_store_rows<T, HDP>(patch, o, inv, p.hd, lane, [&](int r) -> char* {
       const int v = row0 + wave * 32 + r;
       if (v >= vrows) return nullptr;
@@ -238,7 +238,7 @@ template <typename T> __global__ __launch_bounds__(256) void doc_join_kernel(Doc
     const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
     store2(reinterpret_cast<typename T::E*>(p.out) + (size_t)row * p.ld_o + (size_t)head * p.hd + 2 * lane, a0 * inv, a1 * inv);
   }
-  if (lane == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (lane == 0 && p.lse != nullptr) p.lse[(size_t)head * p.rows_q + row] = doc_lse(m, l);
 }
 
 template <typename T, int HDP, int KS, int SHAPE> int run_doc_attn(const DocAttnP& p, hipStream_t st) {

@@ -101,8 +101,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   }
   delta = doc_half_sum(delta);
   const size_t at = (size_t)head * p.rows_q + qrow, n_at = (size_t)p.heads * p.rows_q;
-  const float lse = p.lse[at];
-  const float lse2 = lse == -INFINITY ? INFINITY : lse * kLog2e;  // (no key seen: every p is 0)
+  const float lse2 = doc_lse2(p.lse[at]);
   float slope2 = 0.f;
   if constexpr ((SHAPE & kShapeSlope) != 0) slope2 = p.slopes[head] * kLog2e;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
