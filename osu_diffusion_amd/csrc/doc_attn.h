@@ -240,7 +240,7 @@ __device__ __forceinline__ float doc_half_sum(float v) {
 // tiles under a causal mask come first (the last of its query tiles, the first of its key tiles), so that a launch ends on short ones.
 // Consecutive workgroups sit on consecutive XCDs, so the tiles of a key head stay on the XCDs of its remainder mod 8 and read its keys
 // through their L2s.  (One contiguous eighth of the units per XCD reads each key head through one L2, but where a document's tiles
-// straddle two eighths the later one ends on the longest tile: 2 documents of 8191 positions, 12 / 4 heads of 128 columns, causal: 605 us, in this order 440.)
+// straddle two eighths the later one ends on the longest tile: 2 documents of 8191 positions, 12 / 4 heads of 128 columns, causal: 605 us, in this order 443.)
 struct DocUnit {
   int part, kvh, slot;
 };
@@ -303,7 +303,7 @@ __device__ __forceinline__ int doc_class(const DocAttnP& p, int i0, int i1, int 
 // ---- capped scores.  tanh(x) = 1 - 2 / (1 + e^(2x)) takes two transcendental instructions (16 cycles each; a multiply-add 4).  Where no score of a
 // wave's tile passes half the cap -- the rule outside of outliers -- an odd polynomial of x does: relative error 5.4e-7 with four terms
 // (1.3e-8 with the fifth, for the fp32 tier), a least-maximum fit of tanh(x) / x in x^2 over |x| <= 1/2.  2 documents of 8191 positions, 12 / 4
-// heads of 128 columns, causal: 519 us with the exponential form, 469 with the polynomial.
+// heads of 128 columns, causal: 542 us with the exponential form, 498 with the polynomial.
 template <typename T> __device__ __forceinline__ float doc_tanh_series(const float (&t)[5], float s) {
   const float y = s * s;
   if constexpr (T::kExact) return s * fmaf(y, fmaf(y, fmaf(y, fmaf(y, t[4], t[3]), t[2]), t[1]), t[0]);

@@ -5,7 +5,11 @@
 // the 32 x 32 matrix instructions, so a lane owns one row and the softmax needs one exchange with lane ^ 32; P goes back into the matrix
 // pipe as the B operand without leaving registers; the K | V rows of the next block travel by LDS-DMA into the other half of a double
 // buffer while this block is computed, one barrier per block.  Statistics, sums and accumulators are fp32; P is rounded to the
-// element type for its product (relative 2^-9 in bf16, 2^-12 in fp16: the size of the output's own rounding), its sum is taken before.
+// element type for its product (at most 2^-8 of it in bf16, 2^-11 in fp16: the size of the output's own rounding), its sum is taken before.
+//
+// Bound: the matrix pipe together with the exponentials (16 cycles each, a matrix instruction of 32 x 32 x 16 takes 32).  2 documents of 8192 positions, 12 / 4
+// heads of 128 columns, causal: 443 us, 930 TFLOP/s (a large bf16 product: 1225); 4 documents of 8192, 12 heads of 64: 897 us, 919; one query against
+// 16 x ~8000 keys: 52-60 us, 4.6-5.3 TB/s.
 #include <type_traits>
 
 #include "doc_attn.h"

@@ -4,7 +4,15 @@
 //
 // Two kernels, each recomputing s and dp: the first owns query rows and walks key blocks (dq; it also writes delta and lse * log2(e) for the
 // second), the second owns keys and walks query blocks (dk, dv).  Seven products instead of the five of a single pass, but every sum
-// is taken in a fixed order: no atomics, two runs give the same bits.  p and ds are rounded to the element type for their products.
+// is taken in a fixed order: no atomics, two runs give the same bits.
+//
+// Rounding: p and ds go into p^T d_out and ds^T q in the element type (at most 2^-8 of each in bf16, the size of the results' own rounding).  The
+// delta that the forward's rounded out gives carries that rounding once more, so the first kernel sums p dp on its way and the second uses
+// that; its own product ds k takes ds as two parts, the element type and what that rounded away, to keep the sum of both errors where
+// the other gradients' is (8192 positions with distance penalties, error of dq against 64 bits: 2.3e-3, 2.8e-3 with one part; one rounding: 1.7e-3).
+//
+// Bound: matrix pipe (48 % busy in the first kernel) and the waits for LDS fragments.  8192 positions, 8 / 2 heads of 128 columns, causal: 336 us the first
+// kernel, 320 the second, 20 the join of its parts; 32 documents of 1024 positions, 12 heads of 64: 465 us both.
 #include "doc_attn.h"
 #include "kernels.h"
 

@@ -181,7 +181,7 @@ __device__ __forceinline__ void head(const RopeP& p, bool turn, const float2* cs
 }
 
 // A turn's heads of q, then of k, go by in batches of FL per group of lanes; the next batch is on its way while one is computed, and the first is
-// before the angles are taken: a cold row costs two microseconds.
+// before the angles are taken (32768 rows of 12 + 12 heads of 64 columns, 201 MB not in the caches: 44.7 us, 55.8 with loads where they are used).
 template <typename E, int W, int GL /* lanes per head */, bool INTER, bool BACK>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BACK ? kBackPerCu<W> : 4))) void qk_norm_rope_kernel(RopeP p) {
   constexpr int TPB = kTpb, FL = kFlight<E, BACK>, NG = 256 / GL;
