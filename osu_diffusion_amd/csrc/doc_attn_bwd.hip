@@ -509,7 +509,7 @@ template <typename T> int run_doc_bwd_hd(const DocAttnP& p, hipStream_t st) {
 int doc_bwd_split(const DocAttnP& p, int prec, int max_q) {
   const int tiles = (p.rows_k / 128 + p.n_docs) * p.kv_heads, least = prec == OSUD_PREC_F32 ? 128 : 512;
   const long rows = (long)(max_q > 0 ? max_q : p.rows_q / (p.n_docs > 0 ? p.n_docs : 1)) * p.G;
-  if (tiles <= 0 || tiles > 2 * p.cus) return 1;
+  if (p.rows_k == 0 || tiles <= 0 || tiles > 2 * p.cus) return 1;  // (no keys: nothing to join)
   long n = 4L * p.cus / tiles;
   if (n > rows / least) n = rows / least;
   if (n > 16) n = 16;

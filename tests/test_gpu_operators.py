@@ -467,3 +467,13 @@ def test_leaves_are_refused_inside_a_capture():
             ops.attention(q, q, q, docs)
     eager.sum().backward()
     assert q.grad is not None
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_many_queries_of_documents_without_any_key_row(dtype):
+    """A document that is long on the query side only, and tensors of keys without rows: the backward pass has nothing to split over."""
+    q, none = normal(1, 2100, 2, 64, dtype=dtype), torch.empty(0, 1, 64, device=DEV, dtype=dtype)
+    docs = ops.Documents([2100], device=DEV, kv_lengths=[0])
+    out, lse = ops.attention(q, none, none, docs, return_lse=True)
+    dq, dk, dv = ops.attention_bwd(q, q, none, none, out, lse, docs)
+    assert not bool(out.any()) and bool((lse == -math.inf).all()) and not bool(dq.any()) and dk.shape == dv.shape == none.shape
