@@ -317,7 +317,7 @@ constexpr int kBackGroups = 4 * 256;  // at most so many workgroups in the backw
 template <typename E, int W, int GL, bool INTER, bool BACK> int run_rope(const RopeP& p, hipStream_t st) {
   constexpr int TPB = kTpb;
   const long chunks = p.rows > TPB ? (p.rows + TPB - 1) / TPB : 1;  // (no rows: one workgroup that leaves zeros for the weights)
-  long most = 1L << 30;
+  long most = 1L << 23;  // (a launch has fewer than 2^32 threads; a workgroup takes several turns then)
   if (BACK) {
     most = (long)kBackPerCu<W> * device_cus();
     if (most > kBackGroups) most = kBackGroups;

@@ -477,3 +477,18 @@ def test_many_queries_of_documents_without_any_key_row(dtype):
     out, lse = ops.attention(q, none, none, docs, return_lse=True)
     dq, dk, dv = ops.attention_bwd(q, q, none, none, out, lse, docs)
     assert not bool(out.any()) and bool((lse == -math.inf).all()) and not bool(dq.any()) and dk.shape == dv.shape == none.shape
+
+
+def test_rope_more_rows_than_a_launch_has_threads_for():
+    """2^27 + 13 rows of one small head: every turn of every workgroup, compared where a workgroup's second turn begins and at both ends."""
+    rows, period = (1 << 27) + 13, 4099
+    base = normal(1, period, 1, 2)
+    q = base.repeat(rows // period + 1, 1, 1)[:rows]
+    pos = torch.arange(rows, device=DEV, dtype=torch.int32) % period
+    freqs, _ = ops.rotary_frequencies(2, device=DEV)
+    out, _ = ops.qk_norm_rope(q, None, pos, freqs)
+    one, _ = ops.qk_norm_rope(base, None, pos[:period].contiguous(), freqs)
+    check(one, rope_case(base, None, pos[:period], freqs)["out"], "q")
+    whole = rows // period * period
+    assert bool((out[:whole].view(-1, period, 2).view(torch.int32) == one.view(1, period, 2).view(torch.int32)).all())
+    assert torch.equal(out[whole:], one[:rows - whole])
