@@ -73,9 +73,12 @@ def _call(device, fn, *args):
         _lib.check(rc)
 
 
-def _wants_grad(*tensors):
+def _wants_grad(*tensors, constants=()):
+    """Whether a call records a node; ``constants`` have no gradient (asked here: inside a node's forward grad mode is off)."""
     if not torch.is_grad_enabled():
         return False
+    for name, t in constants:
+        assert t is None or not t.requires_grad, f"{name} have no gradient"
     wants = leaf = False
     for t in tensors:
         if t is not None and t.requires_grad:
@@ -122,7 +125,6 @@ def _rope(q, k, positions, freqs, q_weight, k_weight, norm, eps, interleaved, ga
         krows, r.kv_heads, khd, r.ld_k = _heads("k", k, q)
         assert (krows, khd) == (rows, hd), f"k must have the rows and the head_dim of q, got {tuple(k.shape)} and {tuple(q.shape)}"
     if freqs is not None:
-        assert not (torch.is_grad_enabled() and (freqs.requires_grad or (positions is not None and positions.requires_grad))), "positions and freqs have no gradient"
         r.rot_dim = 2 * freqs.numel()
         r.freqs = _vector("freqs", freqs, freqs.numel(), torch.float64, q.device)
         assert positions is not None and positions.dtype in (torch.int32, torch.float32), "positions must be an int32 or float32 tensor"
@@ -177,7 +179,7 @@ def qk_norm_rope(q, k, positions, freqs, *, q_weight=None, k_weight=None, norm=T
     q (rows, heads, head_dim), k (rows, kv_heads, head_dim) or None; positions (rows,) int32 or float32 (times); freqs float64 from
     ``rotary_frequencies`` or None (norm only); weights (head_dim,) float32 or None.  Returns (q', k'), new tensors or ``out`` (a pair; may be q and k
     themselves), rounded once.  float16 has no gradients."""
-    if _wants_grad(q, k, q_weight, k_weight):
+    if _wants_grad(q, k, q_weight, k_weight, constants=() if freqs is None else (("positions", positions), ("freqs", freqs))):
         assert out is None, "out= cannot be combined with gradients"
         assert q.dtype != torch.float16, "the fp16 tier has no backward pass"
         got = _QkNormRope.apply(q, k, q_weight, k_weight, positions, freqs, norm, eps, interleaved, gain)
@@ -246,7 +248,6 @@ def _attention(q, k, v, docs, scale, cap, left, right, slopes):
     if docs.prefix is not None:
         a.prefix = docs.prefix.data_ptr()
     if slopes is not None:
-        assert not (slopes.requires_grad and torch.is_grad_enabled()), "slopes have no gradient"
         a.slopes = _vector("slopes", slopes, heads, torch.float32, q.device)
     return a
 
@@ -299,7 +300,7 @@ def attention(q, k, v, docs, *, scale=None, cap=0.0, left=None, right=None, slop
     zeros.  Returns out (rows, heads, head_dim), zeros behind the last document (with ``out`` given those rows stay as they are); with ``return_lse``
     also lse (heads, rows) float32, the logarithm of each row's sum of exponentials (-inf: no key), without a gradient.  slopes have no
     gradient; float16 has none at all."""
-    if _wants_grad(q, k, v):
+    if _wants_grad(q, k, v, constants=(("slopes", slopes),)):
         assert out is None, "out= cannot be combined with gradients"
         assert q.dtype != torch.float16, "the fp16 tier has no backward pass"
         got = _Attention.apply(q, k, v, docs, scale, cap, left, right, slopes)

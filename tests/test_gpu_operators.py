@@ -492,3 +492,20 @@ def test_rope_more_rows_than_a_launch_has_threads_for():
     whole = rows // period * period
     assert bool((out[:whole].view(-1, period, 2).view(torch.int32) == one.view(1, period, 2).view(torch.int32)).all())
     assert torch.equal(out[whole:], one[:rows - whole])
+
+
+def test_constants_that_want_a_gradient_are_refused_beside_trained_tensors():
+    """slopes, positions and freqs have no gradient: asking for one raises, also where q, k and v have theirs."""
+    q = normal(1, 10, 2, 64).requires_grad_()
+    docs = ops.Documents([10], device=DEV)
+    slopes = torch.ones(2, device=DEV, requires_grad=True)
+    with pytest.raises(AssertionError):
+        ops.attention(q, q, q, docs, slopes=slopes)
+    freqs, _ = ops.rotary_frequencies(64, device=DEV)
+    times = torch.arange(10, device=DEV).float()
+    with pytest.raises(AssertionError):
+        ops.qk_norm_rope(q, q, times.clone().requires_grad_(), freqs)
+    with pytest.raises(AssertionError):
+        ops.qk_norm_rope(q, q, times, freqs.clone().requires_grad_())
+    with torch.no_grad():  # (nothing is asked for here)
+        ops.attention(q, q, q, docs, slopes=slopes)
