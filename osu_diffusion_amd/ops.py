@@ -166,7 +166,7 @@ class _QkNormRope(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_q, d_k=None):
         q, k, q_weight, k_weight, positions, freqs = ctx.saved_tensors
-        d_q = d_q.contiguous()
+        d_q = d_q.contiguous()  # (rows of any alignment: the norm and rotation take element-aligned pointers)
         d_k = None if k is None else d_k.contiguous()
         dq, dk, dqw, dkw = qk_norm_rope_bwd(d_q, d_k, q, k, positions, freqs, q_weight=q_weight, k_weight=k_weight, **ctx.how)
         return dq, dk, dqw, dkw, None, None, None, None, None, None
@@ -287,7 +287,10 @@ class _Attention(torch.autograd.Function):
         q, k, v, out, lse, slopes = ctx.saved_tensors
         if d_out is None:
             return (None,) * 9
-        return *attention_bwd(d_out.contiguous(), q, k, v, out, lse, ctx.docs, slopes=slopes, **ctx.how), None, None, None, None, None, None
+        d_out = d_out.contiguous()
+        if d_out.data_ptr() % 16:  # (a piece of a larger gradient: the caller cannot choose where it starts)
+            d_out = d_out.clone()
+        return *attention_bwd(d_out, q, k, v, out, lse, ctx.docs, slopes=slopes, **ctx.how), None, None, None, None, None, None
 
 
 def attention(q, k, v, docs, *, scale=None, cap=0.0, left=None, right=None, slopes=None, return_lse=False, out=None):

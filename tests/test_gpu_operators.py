@@ -509,3 +509,21 @@ def test_constants_that_want_a_gradient_are_refused_beside_trained_tensors():
         ops.qk_norm_rope(q, q, times, freqs.clone().requires_grad_())
     with torch.no_grad():  # (nothing is asked for here)
         ops.attention(q, q, q, docs, slopes=slopes)
+
+
+def test_gradients_that_arrive_unaligned():
+    """The upstream gradient as a piece of a longer vector's, one element past 16-byte alignment."""
+    q, k, v = (t.contiguous().requires_grad_() for t in attention_inputs(BF, 2, 2, 64, [20], tail=0))
+    docs = ops.Documents([20], device=DEV)
+    flat = normal(7, 1 + q.numel())
+    d_out = flat[1:].view(q.shape)
+    assert d_out.data_ptr() % 16
+    got = torch.autograd.grad(ops.attention(q, k, v, docs), (q, k, v), d_out)
+    want = torch.autograd.grad(ops.attention(q, k, v, docs), (q, k, v), d_out.clone())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    freqs, _ = ops.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(20, device=DEV, dtype=torch.int32)
+    # (chunks of another width: the same formula, sums in another order; the difference is at most both results' own rounding and fp32 sums)
+    for up in (d_out, d_out.clone()):
+        got = torch.autograd.grad(ops.qk_norm_rope(q, None, pos, freqs)[0], q, up)[0]
+        check(got, rope_case(q.detach(), None, pos, freqs, grad=up)["dx"], "dq")
