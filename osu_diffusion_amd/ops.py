@@ -90,6 +90,15 @@ def _wants_grad(*tensors, constants=()):
     return wants
 
 
+def _written(*tensors):
+    """Tensors that a kernel writes in place of new ones: autograd hears of it, so that a graph which saved their old values raises."""
+    for t in tensors:
+        if t is not None:
+            assert not (t.requires_grad and torch.is_grad_enabled()), "a tensor that requires grad cannot be written to with grad mode on"
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
+
+
 # ------------------------------------------------------------------ norms and rotary positions of queries and keys
 def rotary_frequencies(dim, base=10000.0, *, scaling=None, factor=1.0, original_length=None, device="cuda"):
     """The (dim / 2,) float64 rotary frequencies base^(-2 i / dim), in radians per position, and the gain of the rotated columns.
@@ -145,6 +154,7 @@ def _rope_results(q, k, r, out):
     q_out, k_out = out
     assert q_out.shape == q.shape and (k is None or k_out.shape == k.shape), "out must have the shapes of q and k"
     r.ld_q_out, r.ld_k_out = _heads("out[0]", q_out, q)[3], 0 if k is None else _heads("out[1]", k_out, q)[3]
+    _written(q_out, None if k is None else k_out)
     return q_out, k_out
 
 
@@ -261,6 +271,7 @@ def _attention_forward(q, k, v, docs, a, out):
     else:
         assert out.shape == q.shape, f"out must have the shape of q, got {tuple(out.shape)}"
         a.ld_out = _heads("out", out, q)[3]
+        _written(out)
     lse = torch.empty(q.shape[1], q.shape[0], device=q.device)
     L = _lib.lib()
     n = L.osud_op_doc_attention_ws(C.byref(a), 0)
@@ -300,9 +311,10 @@ def attention(q, k, v, docs, *, scale=None, cap=0.0, left=None, right=None, slop
     to 128.  Query i of a document's nq stands at position nk - nq + i of its nk keys.  Scores: ``scale`` (> 0; 1 / sqrt(head_dim)) times q.k; with ``cap``
     > 0 then cap * tanh(s / cap); with ``slopes`` (heads,) float32 then minus slope * |distance|.  A key is visible within ``left`` positions before
     and ``right`` behind the query's own (None: no bound; right=0: causal), or inside the document's prefix.  A query that sees no key gets
-    zeros.  Returns out (rows, heads, head_dim), zeros behind the last document (with ``out`` given those rows stay as they are); with ``return_lse``
+    zeros.  Returns out (rows, heads, head_dim), zeros behind the last document (with ``out`` given, which must not overlap q, k or v, those rows stay as they are); with ``return_lse``
     also lse (heads, rows) float32, the logarithm of each row's sum of exponentials (-inf: no key), without a gradient.  slopes have no
-    gradient; float16 has none at all."""
+    gradient; float16 has none at all.  What other documents and the rows behind the last one hold has no influence; inside a document k and v
+    must be finite, also where a mask hides them (a hidden NaN may reach the document's other rows, as 0 * NaN)."""
     if _wants_grad(q, k, v, constants=(("slopes", slopes),)):
         assert out is None, "out= cannot be combined with gradients"
         assert q.dtype != torch.float16, "the fp16 tier has no backward pass"
@@ -314,7 +326,7 @@ def attention(q, k, v, docs, *, scale=None, cap=0.0, left=None, right=None, slop
 
 def attention_bwd(d_out, q, k, v, out, lse, docs, *, scale=None, cap=0.0, left=None, right=None, slopes=None, grads=None):
     """Gradients (dq, dk, dv) of ``attention`` for the gradient d_out of its result; out and lse as it returned them.  Rows behind the last
-    document get zeros; with ``grads`` (three tensors to write into, e.g. the parts of one packed gradient) they stay as they are."""
+    document get zeros; with ``grads`` (three tensors to write into, e.g. the parts of one packed gradient; none may overlap an input) they stay as they are."""
     a = _attention(q, k, v, docs, scale, cap, left, right, slopes)
     assert d_out.shape == q.shape and out.shape == q.shape, "d_out and out must have the shape of q"
     assert lse.shape == (q.shape[1], q.shape[0]) and lse.dtype == torch.float32 and lse.device == q.device and lse.is_contiguous(), \
@@ -329,6 +341,7 @@ def attention_bwd(d_out, q, k, v, out, lse, docs, *, scale=None, cap=0.0, left=N
         dq, dk, dv = grads
         assert dq.shape == q.shape and dk.shape == k.shape and dv.shape == v.shape, "grads must have the shapes of q, k and v"
         a.ld_dq, a.ld_dk, a.ld_dv = _heads("dq", dq, q)[3], _heads("dk", dk, q)[3], _heads("dv", dv, q)[3]
+        _written(dq, dk, dv)
     L = _lib.lib()
     n = L.osud_op_doc_attention_ws(C.byref(a), 1)
     ws = torch.empty(max(n, 1), device=q.device)

@@ -527,3 +527,40 @@ def test_gradients_that_arrive_unaligned():
     for up in (d_out, d_out.clone()):
         got = torch.autograd.grad(ops.qk_norm_rope(q, None, pos, freqs)[0], q, up)[0]
         check(got, rope_case(q.detach(), None, pos, freqs, grad=up)["dx"], "dq")
+
+
+def test_results_written_into_given_tensors_are_seen_by_autograd():
+    """A graph that saved the old values raises in its backward; a tensor that requires grad is not written to with grad mode on."""
+    docs = ops.Documents([10], device=DEV)
+    q, k = normal(1, 10, 2, 64), normal(2, 10, 2, 64)
+    freqs, _ = ops.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(10, device=DEV, dtype=torch.int32)
+    with torch.no_grad():
+        out, lse = ops.attention(q, k, k, docs, return_lse=True)
+    writes = [lambda t: ops.qk_norm_rope(t, None, pos, freqs, out=(t, None)), lambda t: ops.attention(q, k, k, docs, out=t),
+              lambda t: ops.attention_bwd(q, q, k, k, out, lse, docs, grads=(torch.empty_like(q), t, torch.empty_like(q)))]
+    for write in writes:
+        leaf = normal(3, 10, 2, 64).requires_grad_()
+        saved = leaf * 1
+        loss = saved.square().sum()
+        with torch.no_grad():
+            write(saved)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+    for write in writes[1:]:
+        with pytest.raises(AssertionError):
+            write(normal(3, 10, 2, 64).requires_grad_())
+    with torch.inference_mode():
+        for write in writes:
+            write(normal(3, 10, 2, 64))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("right", [None, 0])
+def test_slopes_of_either_sign(right, dtype):
+    """Scores that rise with the distance, fall with it, or (0) ignore it: different heads of one call."""
+    lengths, heads = [150, 1, 300], 6
+    q, k, v = attention_inputs(dtype, heads, 2, 64, lengths)
+    d_out = normal(9, q.shape[0], heads, 64, dtype=dtype)
+    slopes = torch.tensor([-0.5, -0.01, 0.0, 0.02, 0.4, 3.0], device=DEV)
+    compare(q, k, v, lengths, d_out=d_out, right=right, slopes=slopes)
