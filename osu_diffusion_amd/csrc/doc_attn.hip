@@ -5,7 +5,7 @@
 // the 32 x 32 matrix instructions, so a lane owns one row and the softmax needs one exchange with lane ^ 32; P goes back into the matrix
 // pipe as the B operand without leaving registers; the K | V rows of the next block travel by LDS-DMA into the other half of a double
 // buffer while this block is computed, one barrier per block.  Statistics, sums and accumulators are fp32; P is rounded to the
-// element type for its product (at most 2^-8 of it in bf16, 2^-11 in fp16: the size of the output's own rounding), its sum is taken before.
+// element type for its product (at most 2^-8 of it in bf16, 2^-11 in fp16: the size of the output's own rounding), the sum of lse is taken before.
 //
 // Bound: the matrix pipe together with the exponentials (16 cycles each, a matrix instruction of 32 x 32 x 16 takes 32).  2 documents of 8192 positions, 12 / 4
 // heads of 128 columns, causal: 443 us, 930 TFLOP/s (a large bf16 product: 1225); 4 documents of 8192, 12 heads of 64: 897 us, 919; one query against
@@ -96,6 +96,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   float m_run = (SHAPE & kShapeFixed) != 0 ? 0.f : -INFINITY, l_run = 0.f;
+  // Without a running maximum a row's largest weight is no power of two and gets rounded, also where it is the only one: the rounded weights' own sum
+  // divides then, and a row that sees one key returns its v
+  constexpr bool kOwnSum = (SHAPE & kShapeFixed) != 0 && !T::kExact;
+  [[maybe_unused]] float l_own = 0.f;
   [[maybe_unused]] const bool onesided = p.right == 0 && d.pre == 0;
 
   const uint32_t kb = lds0 + TL::row_base(lane), vb = lds0 + TILE + TL::tr_base(lane);
@@ -183,6 +187,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
           l_run += e;
         }
         const u32x4 pf = T::pack(s[kt], ss);
+        if constexpr (kOwnSum) l_own = T::sum(pf, l_own);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = T::mma(TL::tr_read(va, kt * 32 + T::STEP * ss, dt, lane), pf, o[dt]);
       }
@@ -190,9 +195,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
   __syncthreads();  // (the stages are idle: they become the waves' patches)
   if (!alive) return;
   const float l = doc_half_sum(l_run);
+  float own = l;
+  if constexpr (kOwnSum) own = doc_half_sum(l_own);
   char* const patch = smem + wave * 32 * TL::RB;
   if (p.split == 1) {
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // (no key seen: zeros)
+    const float inv = own > 0.f || own != own ? 1.0f / own : 0.f;  // (no key seen: zeros)
     if (p.lse != nullptr && half == 0 && vr < vrows)
       p.lse[(size_t)head * p.rows_q + qrow] = doc_lse(m_run, l);
     doc_store_rows<T, HDP>(patch, o, inv, p.hd, lane, [&](int r) -> char* {
@@ -205,6 +212,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(T::ES == 2 
     if (vr < vrows) {
       const size_t at = ((size_t)sp * p.rows_q + qrow) * p.heads + head;
       if (half == 0) *reinterpret_cast<float2*>(p.ws_ml + 2 * at) = make_float2(m_run, l);
+      if constexpr (kOwnSum) {  // (the parts are joined by l)
+        const float f = own > 0.f ? l / own : 1.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -262,7 +276,9 @@ template <typename T, int HDP, int KS> int run_doc_attn_shape(const DocAttnP& p,
   switch ((p.cap > 0.f ? kShapeCap : 0) | (p.slopes != nullptr ? kShapeSlope : 0)) {
     case 0: return run_doc_attn<T, HDP, KS, 0>(p, st);
     case kShapeCap:
-      if (!std::is_same<T, DocF16>::value && p.cap <= kFixedCap) return run_doc_attn<T, HDP, KS, kShapeCap | kShapeFixed>(p, st);
+      if constexpr (!std::is_same<T, DocF16>::value) {
+        if (p.cap <= kFixedCap) return run_doc_attn<T, HDP, KS, kShapeCap | kShapeFixed>(p, st);
+      }
       return run_doc_attn<T, HDP, KS, kShapeCap>(p, st);
     case kShapeSlope: return run_doc_attn<T, HDP, KS, kShapeSlope>(p, st);
     default: return run_doc_attn<T, HDP, KS, kShapeCap | kShapeSlope>(p, st);

@@ -564,3 +564,19 @@ def test_slopes_of_either_sign(right, dtype):
     d_out = normal(9, q.shape[0], heads, 64, dtype=dtype)
     slopes = torch.tensor([-0.5, -0.01, 0.0, 0.02, 0.4, 3.0], device=DEV)
     compare(q, k, v, lengths, d_out=d_out, right=right, slopes=slopes)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("how", [{}, dict(cap=50.0), dict(cap=2.0), dict(cap=90.0), dict(slopes=True), dict(cap=15.0, slopes=True)])
+def test_a_row_that_sees_one_key_returns_its_value(how, dtype):
+    """Its weight is 1 whatever the score: p / sum p differs from 1 by a few fp32 roundings, far less than half a step of the 16-bit type, so v comes back bit
+    for bit -- from documents of one key, a mask of one key, and a long cache whose keys are split over workgroups."""
+    how = dict(how)
+    if how.pop("slopes", False):
+        how["slopes"] = torch.tensor([0.5, 0.01], device=DEV)
+    q, v = normal(1, 300, 2, 96, dtype=dtype), normal(2, 300, 2, 96, dtype=dtype)
+    assert torch.equal(ops.attention(q, q, v, ops.Documents([1] * 300, device=DEV), **how), v)
+    assert torch.equal(ops.attention(q, q, v, ops.Documents([300], device=DEV), left=0, right=0, **how), v)
+    k, v = normal(3, 4100, 2, 96, dtype=dtype), normal(4, 4100, 2, 96, dtype=dtype)
+    docs = ops.Documents([1, 1], device=DEV, kv_lengths=[4000, 100])
+    assert torch.equal(ops.attention(q[:2], k, v, docs, left=0, right=0, **how), v[[3999, 4099]])
